@@ -55,6 +55,10 @@ extern "C" {
 #define Q36MOE_FMT_F32  0
 #define Q36MOE_FMT_BF16 1
 
+/* norms (q36moe_layernorm) */
+#define Q36MOE_NORM_LAYER 0   /* mean taken out  */
+#define Q36MOE_NORM_RMS   1   /* mean left in    */
+
 /* debug taps (q36moe_ctx_copy_tap) */
 #define Q36MOE_TAP_TOPK_IDX  0  /* int32 [T][k]                         */
 #define Q36MOE_TAP_TOPK_W    1  /* f32   [T][k]                         */
@@ -236,6 +240,88 @@ int q36moe_add_rmsnorm_quant(float *h, const float *a, const float *w, int T, in
 int q36moe_forward_q8(q36moe_ctx *c, const q36moe_weights *w, const uint8_t *xq, const uint8_t *xs,
                       const float *logits, int ld_logits, const float *shg, int ld_shg, int T,
                       float scale, void *out, int out_fmt);
+
+/* ---- Training what stands in front of the experts -----------------------
+ * The experts stay as they are; the norm of the MoE input and the router
+ * learn.  No counterpart in the reference, which only infers.  All of these
+ * take device pointers, are asynchronous on `stream`, allocate nothing and
+ * may be captured.  A workspace belongs to the caller: it holds nothing
+ * between calls, needs no clearing, and must not serve two calls that can
+ * run at the same time.  Its size is what the _workspace function gives for
+ * the same sizes (0: ws may be NULL).  Outputs do not overlap inputs, but
+ * where stated.  Sums are fp32; the same call gives the same bits. */
+
+/* Residual add and norm.  Rows of d_model (1..16384) elements, row strides
+ * ld_* >= d_model in elements, any alignment of rows.  For each token t:
+ *   v = x[t] (+ a[t] with a);  h[t] = v (with a; in x's format)
+ *   d = v - mean(v)  (Q36MOE_NORM_RMS: d = v)
+ *   y[t] = d * rsqrt(mean(d^2) + eps) * w + b
+ * x, a, h in x_fmt, y in y_fmt, w and b [d_model] f32 or NULL (1 and 0).
+ * y is formed from the sum before its rounding to h.  h and a go together;
+ * h may be x or a itself, with its stride. */
+int q36moe_layernorm(const void *x, int64_t ld_x, const void *a, int64_t ld_a, int x_fmt, const float *w,
+                     const float *b, int T, int d_model, float eps, int kind, void *h, int64_t ld_h, void *y,
+                     int64_t ld_y, int y_fmt, void *stream);
+
+/* Gradients of the norm of h (the h of q36moe_layernorm, or its x without
+ * an addend; also the h and y of q36moe_add_rmsnorm_quant with
+ * Q36MOE_NORM_RMS): with n = d * rsqrt(mean(d^2) + eps) and g = dy * w,
+ *   dx[t] = rsqrt(..) * (g - mean(g) - n * mean(g * n)) + dres[t]
+ *   dw = sum_t dy[t] * n[t],  db = sum_t dy[t]
+ * (Q36MOE_NORM_RMS: without mean(g)).  dres, the gradient that reaches h by
+ * the residual stream, may be NULL; h, dres and dx are in x_fmt, dy in
+ * y_fmt, w, dw and db [d_model] f32.  Any of dx, dw, db may be NULL, not
+ * all.  The statistics are formed again from h.  T = 0 clears dw and db. */
+size_t q36moe_layernorm_backward_workspace(int T, int d_model);
+int q36moe_layernorm_backward(const void *dy, int64_t ld_dy, int y_fmt, const void *h, int64_t ld_h,
+                              const void *dres, int64_t ld_dres, int x_fmt, const float *w, int T, int d_model,
+                              float eps, int kind, void *dx, int64_t ld_dx, float *dw, float *db, void *ws,
+                              size_t ws_bytes, void *stream);
+
+/* Load of the experts and the loss that balances it.  logits [T][ld] f32,
+ * idx [T][k] as q36moe_router_topk gives it (an index outside
+ * 0..n_expert-1 is a dropped pick and not counted), mask [T] bytes or NULL:
+ * a token with 0 is padding, and nothing of it is read or counted.  With
+ * p = softmax(logits[t]) over the n tokens that are left:
+ *   counts[e] = picks of e,  counts[n_expert] = n,  psum[e] = sum_t p[e]
+ *   loss = coef * n_expert / (k * n^2) * sum_e counts[e] * psum[e]
+ * (0 with n = 0; coef for a perfect balance).  A token whose logits are all
+ * -inf has no probabilities.  counts [n_expert + 1], psum [n_expert] and
+ * loss [1] are written whatever T. */
+size_t q36moe_balance_loss_workspace(int T, int n_expert);
+int q36moe_balance_loss(const float *logits, int ld, const int32_t *idx, const uint8_t *mask, int T, int n_expert,
+                        int k, float coef, int32_t *counts, float *psum, float *loss, void *ws, size_t ws_bytes,
+                        void *stream);
+
+/* Gradient of the router logits, the sum of two parts of which either may
+ * be left out (dwt or counts NULL, not both):
+ *   from the routing weights of q36moe_router_topk (idx, scale and renorm
+ *   as given there), dwt [T][k] their gradient: with q the softmax over the
+ *   token's picks, scale * q_s * (dwt_s - sum_j q_j dwt_j) for pick s;
+ *   without renorm p * (u - sum_e p_e u_e), u_e = scale * dwt of e's pick;
+ *   from the balance loss, counts [n_expert + 1] as q36moe_balance_loss left
+ *   them and dloss its gradient (device pointer, NULL: 1): with
+ *   f = counts / (k * n), dloss * coef * n_expert / n * p * (f - sum_e p_e f_e).
+ *   counts summed over several GPUs first give the loss of all their tokens.
+ * A token with mask 0 gets a row of zeros and nothing of it is read; a pick
+ * outside 0..n_expert-1 takes no part; one that stands twice adds up.
+ * dlogits [T][ld_d], all n_expert columns of each row. */
+int q36moe_router_topk_backward(const float *logits, int ld, const int32_t *idx, const float *dwt,
+                                const int32_t *counts, const uint8_t *mask, const float *dloss, int T,
+                                int n_expert, int k, float scale, int renorm, float coef, float *dlogits, int ld_d,
+                                void *stream);
+
+/* Gradients of q36moe_router_logits (fp32 products and sums, whatever mode
+ * the forward ran in): dlogits [T][ld], and with n_rows == n_expert + 1
+ * dshg, token t's at dshg[t * ld_shg] (ld_shg 0 means 1):
+ *   dw[r] = sum_t dlogits[t][r] * x[t],  dx[t] = sum_r dlogits[t][r] * w[r]
+ * with the shared gate as the last row.  dw [n_rows][d_model] f32, dx
+ * [T][d_model] in x_fmt; either may be NULL (x is read for dw alone, w for
+ * dx alone).  d_model == 2048, T <= 2^25.  T = 0 clears dw. */
+size_t q36moe_router_logits_backward_workspace(int T, int n_rows);
+int q36moe_router_logits_backward(const float *w, int n_rows, int n_expert, const void *x, int x_fmt, int T,
+                                  int d_model, const float *dlogits, int ld, const float *dshg, int ld_shg,
+                                  float *dw, void *dx, void *ws, size_t ws_bytes, void *stream);
 
 /* Execution path of q36moe_forward.  The sorted path (route + sort + grouped
  * expert GEMMs + combine) serves any T, with fat tiles (up to 160 rows per

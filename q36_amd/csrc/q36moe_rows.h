@@ -1,0 +1,159 @@
+// Device helpers shared by the training kernels (q36moe_norm.hip,
+// q36moe_rgrad.hip): row loads and stores in f32 or bf16, reductions over 16
+// and 64 lanes, and the sum of partial rows.
+#ifndef Q36MOE_ROWS_H
+#define Q36MOE_ROWS_H
+#include <hip/hip_runtime.h>
+
+#include <cstddef>
+#include <cstdint>
+
+#include "q36moe.h"
+
+namespace {
+
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+// vectors at element alignment: rows of any width and stride start anywhere,
+// and global loads and stores need no more than that
+typedef float f32x4_u __attribute__((ext_vector_type(4), aligned(4)));
+typedef uint32_t u32x2_u __attribute__((ext_vector_type(2), aligned(2)));
+typedef uint32_t u32x4_u __attribute__((ext_vector_type(4), aligned(2)));
+typedef float f32x2 __attribute__((ext_vector_type(2)));
+typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+
+int hip_status(hipError_t e) { return e == hipSuccess ? Q36MOE_OK : Q36MOE_EHIP; }
+
+__device__ __forceinline__ float bf16_lo(uint32_t u) { return __uint_as_float(u << 16); }
+__device__ __forceinline__ float bf16_hi(uint32_t u) { return __uint_as_float(u & 0xffff0000u); }
+// two floats to bf16, round to nearest even (v_cvt_pk_bf16_f32)
+__device__ __forceinline__ uint32_t bf16_pair(float a, float b) {
+    return __builtin_bit_cast(uint32_t, __builtin_convertvector((f32x2{a, b}), bf16x2));
+}
+
+// N consecutive elements (1, 4 or 8) of a row in format F, as floats.
+template <int F, int N>
+__device__ __forceinline__ void load_row(const void *p, size_t at, float (&v)[N]) {
+    if constexpr (F == Q36MOE_FMT_F32) {
+        const float *f = static_cast<const float *>(p) + at;
+        if constexpr (N == 1) {
+            v[0] = *f;
+        } else {
+#pragma unroll
+            for (int i = 0; i < N; i += 4) {
+                const f32x4 t = *reinterpret_cast<const f32x4_u *>(f + i);
+#pragma unroll
+                for (int j = 0; j < 4; j++) v[i + j] = t[j];
+            }
+        }
+    } else {
+        const uint16_t *h = static_cast<const uint16_t *>(p) + at;
+        if constexpr (N == 1) {
+            v[0] = __uint_as_float((uint32_t)*h << 16);
+        } else if constexpr (N == 4) {
+            const u32x2_u t = *reinterpret_cast<const u32x2_u *>(h);
+            v[0] = bf16_lo(t[0]); v[1] = bf16_hi(t[0]); v[2] = bf16_lo(t[1]); v[3] = bf16_hi(t[1]);
+        } else {
+            const u32x4_u t = *reinterpret_cast<const u32x4_u *>(h);
+#pragma unroll
+            for (int j = 0; j < 4; j++) { v[2 * j] = bf16_lo(t[j]); v[2 * j + 1] = bf16_hi(t[j]); }
+        }
+    }
+}
+
+template <int F>
+__device__ __forceinline__ void store_one(void *p, size_t at, float v) {
+    if constexpr (F == Q36MOE_FMT_F32) static_cast<float *>(p)[at] = v;
+    else static_cast<uint16_t *>(p)[at] = (uint16_t)bf16_pair(v, 0.0f);
+}
+
+// The elements from..N-1 of v to at.. (all of them in one or two stores).
+template <int F, int N>
+__device__ __forceinline__ void store_row(void *p, size_t at, const float (&v)[N], int from) {
+    if (N == 1 || from) {
+#pragma unroll
+        for (int i = 0; i < N; i++)
+            if (i >= from) store_one<F>(p, at + i, v[i]);
+        return;
+    }
+    if constexpr (F == Q36MOE_FMT_F32) {
+        float *f = static_cast<float *>(p) + at;
+#pragma unroll
+        for (int i = 0; i + 3 < N; i += 4) *reinterpret_cast<f32x4_u *>(f + i) = f32x4{v[i], v[i + 1], v[i + 2], v[i + 3]};
+    } else {
+        uint16_t *h = static_cast<uint16_t *>(p) + at;
+        if constexpr (N == 4)
+            *reinterpret_cast<u32x2_u *>(h) = u32x2_u{bf16_pair(v[0], v[1]), bf16_pair(v[2], v[3])};
+        else if constexpr (N == 8)
+            *reinterpret_cast<u32x4_u *>(h) = u32x4_u{bf16_pair(v[0], v[1]), bf16_pair(v[2], v[3]),
+                                                      bf16_pair(v[4], v[5]), bf16_pair(v[6], v[7])};
+    }
+}
+
+template <int CTRL>
+__device__ __forceinline__ float dpp(float v) {
+    return __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), CTRL, 0xf, 0xf, false));
+}
+
+// Sum (maximum) over each row of 16 lanes, the same bits in all of them: quad
+// xor 1, quad xor 2, half-row mirror, row mirror.
+__device__ __forceinline__ float sum16(float v) {
+    v += dpp<0xB1>(v);
+    v += dpp<0x4E>(v);
+    v += dpp<0x141>(v);
+    return v + dpp<0x140>(v);
+}
+__device__ __forceinline__ float max16(float v) {
+    v = fmaxf(v, dpp<0xB1>(v));
+    v = fmaxf(v, dpp<0x4E>(v));
+    v = fmaxf(v, dpp<0x141>(v));
+    return fmaxf(v, dpp<0x140>(v));
+}
+
+// Sum over lanes l, l^16, l^32, l^48 (v_permlane16_swap / v_permlane32_swap put
+// the halves side by side), and over the whole wave; all lanes get the same bits.
+__device__ __forceinline__ float sum_rows4(float a) {
+    const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(a), __float_as_uint(a), false, false);
+    a = __uint_as_float(r[0]) + __uint_as_float(r[1]);
+    const auto t = __builtin_amdgcn_permlane32_swap(__float_as_uint(a), __float_as_uint(a), false, false);
+    return __uint_as_float(t[0]) + __uint_as_float(t[1]);
+}
+__device__ __forceinline__ float sum64(float v) { return sum_rows4(sum16(v)); }
+
+// out[c] = sum over p < P of part[p * L + c], in the order of 16 interleaved
+// groups; columns from `split` on go to out2.  64 columns per workgroup: each
+// thread adds a sixteenth of the rows of 4 of them.
+constexpr int kSumCols = 64;
+__global__ __launch_bounds__(256) void k_sum_partials(const float *__restrict__ part, int P, size_t L, size_t split,
+                                                      float *__restrict__ out, float *__restrict__ out2) {
+    __shared__ __align__(16) float red[16][kSumCols];
+    const int c4 = (threadIdx.x & 15) * 4, g = threadIdx.x >> 4;
+    const size_t c = (size_t)blockIdx.x * kSumCols + c4;
+    f32x4 acc = {0.f, 0.f, 0.f, 0.f};
+    if (c + 4 <= L) {
+#pragma unroll 4
+        for (int p = g; p < P; p += 16) acc += *reinterpret_cast<const f32x4_u *>(part + (size_t)p * L + c);
+    } else {
+        for (int p = g; p < P; p += 16)
+#pragma unroll
+            for (int i = 0; i < 4; i++)
+                if (c + i < L) acc[i] += part[(size_t)p * L + c + i];
+    }
+    *reinterpret_cast<f32x4 *>(&red[g][c4]) = acc;
+    __syncthreads();
+    if (threadIdx.x < kSumCols) {
+        const size_t o = (size_t)blockIdx.x * kSumCols + threadIdx.x;
+        float s = red[0][threadIdx.x];
+#pragma unroll
+        for (int i = 1; i < 16; i++) s += red[i][threadIdx.x];
+        if (o < split) out[o] = s;
+        else if (o < L) out2[o - split] = s;
+    }
+}
+
+inline void sum_partials(const float *part, int P, size_t L, size_t split, float *out, float *out2, hipStream_t s) {
+    hipLaunchKernelGGL(k_sum_partials, dim3((unsigned)((L + kSumCols - 1) / kSumCols)), dim3(256), 0, s, part, P, L, split,
+                       out, out2);
+}
+
+}  // namespace
+#endif

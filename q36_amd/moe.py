@@ -18,6 +18,7 @@ LIB_PATH = os.path.join(_HERE, "libq36moe.so")
 
 FMT_F32 = 0
 FMT_BF16 = 1
+NORM_LAYER, NORM_RMS = 0, 1
 
 TAP_TOPK_IDX, TAP_TOPK_W, TAP_XQ, TAP_XS, TAP_EOFF, TAP_PERM, TAP_POS, TAP_HQ, TAP_HS, TAP_DNW = range(10)
 TAP_HSF, TAP_XQ8, TAP_XSF = 10, 11, 12
@@ -70,6 +71,15 @@ def lib():
     L.q36moe_add_rmsnorm_quant.argtypes = [vp, vp, vp, i, i, f, vp, vp, vp, vp]
     L.q36moe_forward_q8.argtypes = [vp, vp, vp, vp, vp, i, vp, i, i, f, vp, i]
     L.q36moe_forward_noalloc.argtypes = [vp, vp, i, vp, i, vp, i, i, i, f, vp, i, vp]
+    i64 = ctypes.c_int64
+    L.q36moe_layernorm.argtypes = [vp, i64, vp, i64, i, vp, vp, i, i, f, i, vp, i64, vp, i64, i, vp]
+    L.q36moe_layernorm_backward.argtypes = [vp, i64, i, vp, i64, vp, i64, i, vp, i, i, f, i, vp, i64, vp, vp, vp, sz, vp]
+    L.q36moe_balance_loss.argtypes = [vp, i, vp, vp, i, i, i, f, vp, vp, vp, vp, sz, vp]
+    L.q36moe_router_topk_backward.argtypes = [vp, i, vp, vp, vp, vp, vp, i, i, i, f, i, f, vp, i, vp]
+    L.q36moe_router_logits_backward.argtypes = [vp, i, i, vp, i, i, i, vp, i, vp, i, vp, vp, vp, sz, vp]
+    for name in ("layernorm_backward", "balance_loss", "router_logits_backward"):
+        fn = getattr(L, f"q36moe_{name}_workspace")
+        fn.argtypes, fn.restype = [i, i], sz
     L.q36moe_ctx_copy_tap.argtypes = [vp, i, vp, sz, ctypes.POINTER(sz)]
     L.q36moe_ctx_set_path.argtypes = [vp, i]
     L.q36moe_ctx_last_path.argtypes = [vp]
@@ -564,6 +574,193 @@ def quant_e4m3(x):
     check(lib().q36moe_quant_e4m3(xp, fmt, T, K, xq.data_ptr(),
                                   xs.data_ptr(), _stream()), "q36moe_quant_e4m3")
     return xq, xs
+
+
+# ---------------------------------------------------------------------------
+# training what stands in front of the experts
+# ---------------------------------------------------------------------------
+_FMT = {torch.float32: FMT_F32, torch.bfloat16: FMT_BF16}
+
+
+def _rows(t, name, shape, dtypes, dev):
+    """(pointer, row stride) of a 2-D GPU tensor of `shape` on device `dev`
+    whose rows are contiguous and do not overlap."""
+    if not isinstance(t, torch.Tensor) or t.device != dev:
+        raise Q36MoEError(f"{name} must be a tensor on {dev}")
+    if t.dtype not in dtypes:
+        raise Q36MoEError(f"{name} must be {' or '.join(map(str, dtypes))}, got {t.dtype}")
+    if t.dim() != 2 or t.shape != shape:
+        raise Q36MoEError(f"{name} must be {list(shape)}, got {list(t.shape)}")
+    T, n = shape
+    if n > 1 and t.stride(1) != 1:
+        raise Q36MoEError(f"{name} rows must be contiguous")
+    if T < 2:
+        return t.data_ptr(), n
+    if t.stride(0) < n:
+        raise Q36MoEError(f"{name} rows must not overlap")
+    return t.data_ptr(), t.stride(0)
+
+
+def _vec(t, name, n, dtypes, dev):
+    """Pointer of a contiguous 1-D GPU tensor of n elements, or None."""
+    if t is None:
+        return None
+    if not isinstance(t, torch.Tensor) or t.device != dev or t.dtype not in dtypes or t.shape != (n,) or \
+            not t.is_contiguous():
+        raise Q36MoEError(f"{name} must be a contiguous {dtypes[0]} tensor of {n} elements on {dev}")
+    return t.data_ptr()
+
+
+def _current(t, name, dims=2):
+    """The device of `t`, which must be the current one: kernels are launched there."""
+    if not isinstance(t, torch.Tensor) or not t.is_cuda:
+        raise Q36MoEError(f"{name} must be a GPU tensor")
+    if t.dim() != dims:
+        raise Q36MoEError(f"{name} must have {dims} dimensions")
+    if t.device.index != torch.cuda.current_device():
+        raise Q36MoEError(f"{name} is on {t.device}, the current device is cuda:{torch.cuda.current_device()}")
+    return t.device
+
+
+def _workspace(n, dev):
+    return torch.empty(n, dtype=torch.uint8, device=dev) if n else None
+
+
+def _ptr(t):
+    return None if t is None else t.data_ptr()
+
+
+def layernorm(x, w=None, b=None, a=None, eps=1e-6, rms=False, out_dtype=None):
+    """Residual add + layer norm (rms: RMS norm) of rows: x, a [T, D] f32|bf16
+    (rows contiguous, any row stride), w, b [D] f32 or None -> (y, h): y [T, D]
+    in out_dtype (x's if None), h = x + a in x's dtype (None without a)."""
+    dev = _current(x, "x")
+    T, D = x.shape
+    xp, ldx = _rows(x, "x", (T, D), tuple(_FMT), dev)
+    ap, lda = (None, D) if a is None else _rows(a, "a", (T, D), (x.dtype,), dev)
+    out_dtype = out_dtype or x.dtype
+    if out_dtype not in _FMT:
+        raise Q36MoEError("out_dtype must be float32 or bfloat16")
+    wp, bp = _vec(w, "w", D, (torch.float32,), dev), _vec(b, "b", D, (torch.float32,), dev)
+    y = torch.empty((T, D), dtype=out_dtype, device=dev)
+    h = None if a is None else torch.empty((T, D), dtype=x.dtype, device=dev)
+    check(lib().q36moe_layernorm(xp, ldx, ap, lda, _FMT[x.dtype], wp, bp, T, D, float(eps),
+                                 NORM_RMS if rms else NORM_LAYER, _ptr(h), D, y.data_ptr(), D, _FMT[out_dtype],
+                                 _stream()), "q36moe_layernorm")
+    return y, h
+
+
+def layernorm_backward(dy, h, w=None, dres=None, eps=1e-6, rms=False, want_dx=True, want_dw=True, want_db=None):
+    """Gradients of layernorm's y: dy [T, D] f32|bf16, h [T, D] f32|bf16 (the
+    normalised rows: layernorm's h, or its x without an addend), dres [T, D]
+    (the residual stream's gradient, added to dx) or None -> (dx, dw, db): dx
+    [T, D] in h's dtype, dw and db [D] f32; None for what is not wanted (db is,
+    by default, for a layer norm)."""
+    dev = _current(h, "h")
+    T, D = h.shape
+    hp, ldh = _rows(h, "h", (T, D), tuple(_FMT), dev)
+    gp, ldg = _rows(dy, "dy", (T, D), tuple(_FMT), dev)
+    rp, ldr = (None, D) if dres is None else _rows(dres, "dres", (T, D), (h.dtype,), dev)
+    wp = _vec(w, "w", D, (torch.float32,), dev)
+    dx = torch.empty((T, D), dtype=h.dtype, device=dev) if want_dx else None
+    dw = torch.empty((D,), dtype=torch.float32, device=dev) if want_dw else None
+    db = torch.empty((D,), dtype=torch.float32, device=dev) if (not rms if want_db is None else want_db) else None
+    L = lib()
+    n = L.q36moe_layernorm_backward_workspace(T, D) if want_dw or db is not None else 0
+    ws = _workspace(n, dev)
+    check(L.q36moe_layernorm_backward(gp, ldg, _FMT[dy.dtype], hp, ldh, rp, ldr, _FMT[h.dtype], wp, T, D, float(eps),
+                                      NORM_RMS if rms else NORM_LAYER, _ptr(dx), D, _ptr(dw), _ptr(db), _ptr(ws), n,
+                                      _stream()), "q36moe_layernorm_backward")
+    return dx, dw, db
+
+
+def _mask(mask, T, dev):
+    """Pointer of the tokens' mask (bool or uint8, 0 for padding), or None."""
+    return _vec(mask, "mask", T, (torch.uint8, torch.bool), dev)
+
+
+def _picks(idx, T, dev):
+    p, _ = _rows(idx, "idx", (T, idx.shape[1] if isinstance(idx, torch.Tensor) and idx.dim() == 2 else -1), (torch.int32,), dev)
+    if not idx.is_contiguous():
+        raise Q36MoEError("idx must be contiguous")
+    return p
+
+
+def balance_loss(logits, idx, coef=1.0, mask=None, n_expert=None):
+    """Load of the experts and the loss that balances it: logits [T, >=n_expert]
+    f32 (row stride free), idx [T, k] int32 (router_topk's), mask [T] bool|uint8
+    (0 for padding) or None -> (loss [] f32, counts int32 [n_expert + 1], the
+    last one the number of live tokens, psum f32 [n_expert], the sums of the
+    tokens' softmax)."""
+    dev = _current(logits, "logits")
+    T = logits.shape[0]
+    E = n_expert or logits.shape[1]
+    lp, ld = _rows(logits, "logits", tuple(logits.shape), (torch.float32,), dev)
+    ip, mp = _picks(idx, T, dev), _mask(mask, T, dev)
+    loss = torch.empty((), dtype=torch.float32, device=dev)
+    counts = torch.empty((E + 1,), dtype=torch.int32, device=dev)
+    psum = torch.empty((E,), dtype=torch.float32, device=dev)
+    L = lib()
+    n = L.q36moe_balance_loss_workspace(T, E)
+    ws = _workspace(n, dev)
+    check(L.q36moe_balance_loss(lp, ld, ip, mp, T, E, idx.shape[1], float(coef), counts.data_ptr(), psum.data_ptr(),
+                                loss.data_ptr(), _ptr(ws), n, _stream()), "q36moe_balance_loss")
+    return loss, counts, psum
+
+
+def router_topk_backward(logits, idx, dwt=None, scale=1.0, renorm=True, counts=None, coef=1.0, mask=None, dloss=None,
+                         n_expert=None):
+    """Gradient of the router logits -> f32 [T, n_expert]: from dwt [T, k] f32,
+    the gradient of router_topk's weights (scale and renorm as there), and, with
+    the counts of balance_loss, from its loss (coef as there, dloss [] f32 its
+    gradient, 1 if None).  Rows with mask 0 are zero."""
+    dev = _current(logits, "logits")
+    T = logits.shape[0]
+    E = n_expert or logits.shape[1]
+    lp, ld = _rows(logits, "logits", tuple(logits.shape), (torch.float32,), dev)
+    ip, mp = _picks(idx, T, dev), _mask(mask, T, dev)
+    k = idx.shape[1]
+    wp = None
+    if dwt is not None:
+        wp, _ = _rows(dwt, "dwt", (T, k), (torch.float32,), dev)
+        if not dwt.is_contiguous():
+            raise Q36MoEError("dwt must be contiguous")
+    cp = _vec(counts, "counts", E + 1, (torch.int32,), dev)
+    if dloss is not None and (not isinstance(dloss, torch.Tensor) or dloss.device != dev or dloss.dtype != torch.float32 or
+                              dloss.numel() != 1):
+        raise Q36MoEError(f"dloss must be one float32 value on {dev}")
+    out = torch.empty((T, E), dtype=torch.float32, device=dev)
+    check(lib().q36moe_router_topk_backward(lp, ld, ip, wp, cp, mp, _ptr(dloss), T, E, k, float(scale), 1 if renorm else 0,
+                                            float(coef), out.data_ptr(), E, _stream()), "q36moe_router_topk_backward")
+    return out
+
+
+def router_logits_backward(w, x, n_expert, dlogits, dshg=None, want_dw=True, want_dx=True):
+    """Gradients of router_logits: w [n_rows, 2048] f32, x [T, 2048] f32|bf16,
+    dlogits [T, n_expert] f32 (row stride free) and, with n_rows == n_expert + 1,
+    dshg [T] f32 (any stride) -> (dw f32 [n_rows, 2048], dx [T, 2048] in x's
+    dtype; None for what is not wanted)."""
+    dev = _current(x, "x")
+    T, D = x.shape
+    n_rows = w.shape[0]
+    wp, _ = _rows(w, "w", (n_rows, D), (torch.float32,), dev)
+    xp, _ = _rows(x, "x", (T, D), tuple(_FMT), dev)
+    if not (w.is_contiguous() and x.is_contiguous()):
+        raise Q36MoEError("w and x must be contiguous")
+    gp, ld = _rows(dlogits, "dlogits", (T, n_expert), (torch.float32,), dev)
+    if (dshg is None) != (n_rows == n_expert):
+        raise Q36MoEError("dshg goes with the shared gate's row")
+    if dshg is not None and dshg.device != dev:
+        raise Q36MoEError(f"dshg must be on {dev}")
+    sp, lds = _shg(dshg, T)
+    dw = torch.empty((n_rows, D), dtype=torch.float32, device=dev) if want_dw else None
+    dx = torch.empty((T, D), dtype=x.dtype, device=dev) if want_dx else None
+    L = lib()
+    n = L.q36moe_router_logits_backward_workspace(T, n_rows) if want_dw else 0
+    ws = _workspace(n, dev)
+    check(L.q36moe_router_logits_backward(wp, n_rows, n_expert, xp, _FMT[x.dtype], T, D, gp, ld, sp, lds, _ptr(dw),
+                                          _ptr(dx), _ptr(ws), n, _stream()), "q36moe_router_logits_backward")
+    return dw, dx
 
 
 def probe_mfma(a, b, sa, sb, fmt_a, fmt_b):
