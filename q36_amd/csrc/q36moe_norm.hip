@@ -241,7 +241,15 @@ __global__ __launch_bounds__(NW == 1 ? 256 : 64 * NW) void k_layernorm_backward(
 constexpr int kWaveRow = 512;
 constexpr int kMaxStreams = 512;   // streams of the backward pass, each with a row of partial sums
 
-int streams(int T) { return T < kMaxStreams ? T : kMaxStreams; }
+// A row each up to 256 tokens, then 4 rows and more: a stream's partial row is
+// written and read again, as much as half a token's own traffic.  Past 256 a
+// multiple of 4: the four waves of a workgroup are streams where NW is 1, and
+// every one of them has rows.
+int streams(int T) {
+    if (T <= kMaxStreams / 2) return T;
+    const int n = (int)(((int64_t)T + 15) / 16) * 4;
+    return n < kMaxStreams / 2 ? kMaxStreams / 2 : n < kMaxStreams ? n : kMaxStreams;
+}
 
 template <bool BWD, int XF, int YF, int VEC, int NW, int NV>
 void launch_norm(const NormArgs &A, hipStream_t s) {

@@ -12,9 +12,18 @@
 //   router product      dW = dlogits^T x,  dx = dlogits W
 #include "q36moe_rows.h"
 
+#include <type_traits>
+
 namespace {
 
 constexpr int kMaxE = 256, kMaxK = 8;
+
+// A wave's LDS writes before its reads.
+__device__ __forceinline__ void wave_sync() {
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+}
 
 // exp(x) for x <= 0 as 2^hi * (1 + lo ln 2), hi + lo = x log2(e) to 48 bits:
 // about 1 ulp however large -x is.
@@ -27,33 +36,81 @@ __device__ __forceinline__ float exp_neg(float x) {
     return e == 0.0f ? 0.0f : fmaf(e, lo * 0.693147180559945309417f, e);
 }
 
-// Softmax of a token's logits by 16 lanes; lane l holds experts l + 16 i, -inf
-// past the last one.  A row of -inf has no probabilities: all 0.
-template <int NI>
-__device__ __forceinline__ void softmax16(float (&v)[NI]) {
-    float m = v[0];
+// A token's E values in 16 lanes: lane l holds columns 64 i + 4 l..+3 in v[i],
+// so that rows move as 16-byte vectors where E is a multiple of 4 (whatever
+// their alignment) and as single values elsewhere.  Columns past E read as
+// `fill`.
+template <int NV>
+__device__ __forceinline__ void load16(const float *__restrict__ row, int E, int l, float fill, float (&v)[NV][4]) {
+    if ((E & 3) == 0) {
 #pragma unroll
-    for (int i = 1; i < NI; i++) m = fmaxf(m, v[i]);
+        for (int i = 0; i < NV; i++) load_row<Q36MOE_FMT_F32>(row, min(64 * i + 4 * l, E - 4), v[i]);
+#pragma unroll
+        for (int i = 0; i < NV; i++)
+#pragma unroll
+            for (int c = 0; c < 4; c++) v[i][c] = 64 * i + 4 * l < E ? v[i][c] : fill;
+    } else {
+#pragma unroll
+        for (int i = 0; i < NV; i++)
+#pragma unroll
+            for (int c = 0; c < 4; c++) v[i][c] = row[min(64 * i + 4 * l + c, E - 1)];
+#pragma unroll
+        for (int i = 0; i < NV; i++)
+#pragma unroll
+            for (int c = 0; c < 4; c++) v[i][c] = 64 * i + 4 * l + c < E ? v[i][c] : fill;
+    }
+}
+
+template <int NV>
+__device__ __forceinline__ void store16(float *__restrict__ row, int E, int l, const float (&v)[NV][4]) {
+    if ((E & 3) == 0) {
+#pragma unroll
+        for (int i = 0; i < NV; i++)
+            if (64 * i + 4 * l < E) store_row<Q36MOE_FMT_F32>(row, 64 * i + 4 * l, v[i], 0);
+    } else {
+#pragma unroll
+        for (int i = 0; i < NV; i++)
+#pragma unroll
+            for (int c = 0; c < 4; c++)
+                if (64 * i + 4 * l + c < E) row[64 * i + 4 * l + c] = v[i][c];
+    }
+}
+
+// Softmax of the values that 16 lanes hold; m and s are left to the caller.  A
+// row of -inf has no probabilities: all 0.
+template <int NV, int NC>
+__device__ __forceinline__ void softmax16(float (&v)[NV][NC]) {
+    float m = v[0][0];
+#pragma unroll
+    for (int i = 0; i < NV; i++)
+#pragma unroll
+        for (int c = 0; c < NC; c++) m = fmaxf(m, v[i][c]);
     m = max16(m);
     m = m == -INFINITY ? 0.0f : m;
     float s = 0.0f;
 #pragma unroll
-    for (int i = 0; i < NI; i++) {
-        v[i] = exp_neg(v[i] - m);
-        s += v[i];
-    }
+    for (int i = 0; i < NV; i++)
+#pragma unroll
+        for (int c = 0; c < NC; c++) {
+            v[i][c] = exp_neg(v[i][c] - m);
+            s += v[i][c];
+        }
     s = sum16(s);
     const float inv = s == 0.0f ? 0.0f : 1.0f / s;   // a NaN stays one
 #pragma unroll
-    for (int i = 0; i < NI; i++) v[i] *= inv;
+    for (int i = 0; i < NV; i++)
+#pragma unroll
+        for (int c = 0; c < NC; c++) v[i][c] *= inv;
 }
 
-template <int NI>
-__device__ __forceinline__ void load_logits(const float *__restrict__ row, int E, int l, float (&v)[NI]) {
+template <int NV>
+__device__ __forceinline__ float dot16(const float (&a)[NV][4], const float (&b)[NV][4]) {
+    float d = 0.0f;
 #pragma unroll
-    for (int i = 0; i < NI; i++) v[i] = row[min(l + 16 * i, E - 1)];
+    for (int i = 0; i < NV; i++)
 #pragma unroll
-    for (int i = 0; i < NI; i++) v[i] = l + 16 * i < E ? v[i] : -INFINITY;
+        for (int c = 0; c < 4; c++) d = fmaf(a[i][c], b[i][c], d);
+    return sum16(d);
 }
 
 // ---------------------------------------------------------------------------
@@ -67,108 +124,122 @@ struct BalanceArgs {
     float coef;
     int32_t *counts;           // [E + 1]
     float *psum, *loss;        // [E], [1]
-    float *part;               // [workgroups][E] sums, then [workgroups][E + 1] counts
+    float2 *part;              // [workgroups][E + 1]: sum of probabilities, count
 };
 
-// loss from counts and sums by one workgroup, in 64 bits: counts times sums of
+// loss from counts and sums by the first wave, in 64 bits: counts times sums of
 // probabilities over many tokens.
-__device__ __forceinline__ void balance_of(const BalanceArgs &A, const int32_t *cnt, const float *ps, double *red) {
+__device__ __forceinline__ void balance_of(const BalanceArgs &A, const int32_t *cnt, const float *ps) {
     if (threadIdx.x < 64) {
         double s = 0.0;
-        for (int e = threadIdx.x; e < A.E; e += 64) s += (double)cnt[e] * (double)ps[e];
-        red[threadIdx.x] = s;
-    }
-    __syncthreads();
-    if (threadIdx.x == 0) {
-        double s = 0.0;
-        for (int i = 0; i < 64; i++) s += red[i];
+#pragma unroll
+        for (int i = 0; i < kMaxE / 64; i++) {
+            const int e = threadIdx.x + 64 * i;
+            if (e < A.E) s += (double)cnt[e] * (double)ps[e];
+        }
+#pragma unroll
+        for (int o = 32; o > 0; o >>= 1) s += __shfl_xor(s, o, 64);
         const double n = (double)cnt[A.E];
-        *A.loss = n > 0.0 ? (float)((double)A.coef * A.E * s / ((double)A.k * n * n)) : 0.0f;
+        if (threadIdx.x == 0) *A.loss = n > 0.0 ? (float)((double)A.coef * A.E * s / ((double)A.k * n * n)) : 0.0f;
     }
 }
 
 constexpr int kBalW = 16;   // waves per workgroup
 
-// 16 lanes per token, 64 tokens of the workgroup's run at a time.
-template <int NI>
+// 16 lanes per token, 64 tokens of the workgroup's run at a time, the next
+// token's loads ahead of the sums of this one.  A token of padding is a row of
+// -inf without picks.
+template <int NV>
 __global__ __launch_bounds__(64 * kBalW) void k_balance(BalanceArgs A) {
-    __shared__ float ps[kBalW][16 * NI];
+    __shared__ __align__(16) float ps[kBalW][64 * NV];
     __shared__ int32_t cnt[kMaxE + 1];
-    __shared__ double red[64];
     const int tid = threadIdx.x, l = tid & 15, wave = tid >> 6;
     const int64_t t0 = (int64_t)blockIdx.x * A.chunk, t1 = min(t0 + A.chunk, (int64_t)A.T);
     for (int e = tid; e <= A.E; e += 64 * kBalW) cnt[e] = 0;
-    float acc[NI];
-#pragma unroll
-    for (int i = 0; i < NI; i++) acc[i] = 0.0f;
-    for (int64_t t = t0 + (tid >> 4); t < t1; t += 4 * kBalW) {
-        if (A.mask && !A.mask[t]) continue;
-        float v[NI];
-        load_logits(A.logits + (size_t)t * A.ld, A.E, l, v);
-        softmax16(v);
-#pragma unroll
-        for (int i = 0; i < NI; i++) acc[i] += v[i];
-    }
-    __syncthreads();   // cnt cleared
-    int live = 0;
-    for (int64_t t = t0 + tid; t < t1; t += 64 * kBalW) {
-        if (A.mask && !A.mask[t]) continue;
-        live++;
-        for (int s = 0; s < A.k; s++) {
-            const int e = A.idx[(size_t)t * A.k + s];
-            if ((unsigned)e < (unsigned)A.E) atomicAdd(&cnt[e], 1);
+    __syncthreads();
+    float acc[NV][4] = {}, v[NV][4];
+    int pick = -1, n = 0;
+    bool live = false;
+    auto load = [&](int64_t t) {
+        live = t < t1;
+        const int64_t tc = min(t, t1 - 1);   // a run without tokens has no logits to read
+        if (tc >= t0) {
+            load16(A.logits + (size_t)tc * A.ld, A.E, l, -INFINITY, v);
+            pick = l < A.k ? A.idx[(size_t)tc * A.k + l] : -1;
+            if (A.mask) live = live && A.mask[tc];
         }
-    }
-    if (live) atomicAdd(&cnt[A.E], live);
+    };
+    int64_t t = t0 + (tid >> 4);
+    load(t);
+    for (; t < t1; t += 4 * kBalW) {
+        float p[NV][4];
 #pragma unroll
-    for (int i = 0; i < NI; i++) {
-        const float s = sum_rows4(acc[i]);
-        if ((tid & 63) < 16) ps[wave][l + 16 * i] = s;
+        for (int i = 0; i < NV; i++)
+#pragma unroll
+            for (int c = 0; c < 4; c++) p[i][c] = live ? v[i][c] : -INFINITY;
+        if (live) {
+            if ((unsigned)pick < (unsigned)A.E) atomicAdd(&cnt[pick], 1);
+            n += l == 0;
+        }
+        load(t + 4 * kBalW);
+        softmax16(p);
+#pragma unroll
+        for (int i = 0; i < NV; i++)
+#pragma unroll
+            for (int c = 0; c < 4; c++) acc[i][c] += p[i][c];
+    }
+    if (n) atomicAdd(&cnt[A.E], n);
+#pragma unroll
+    for (int i = 0; i < NV; i++) {
+#pragma unroll
+        for (int c = 0; c < 4; c++) acc[i][c] = sum_rows4(acc[i][c]);
+        if ((tid & 63) < 16) *reinterpret_cast<float4 *>(&ps[wave][64 * i + 4 * l]) = make_float4(acc[i][0], acc[i][1], acc[i][2], acc[i][3]);
     }
     __syncthreads();
-    const bool all = gridDim.x == 1;
-    float *po = all ? A.psum : A.part + (size_t)blockIdx.x * A.E;
-    int32_t *co = all ? A.counts
-                      : reinterpret_cast<int32_t *>(A.part + (size_t)gridDim.x * A.E) + (size_t)blockIdx.x * (A.E + 1);
-    for (int e = tid; e < A.E; e += 64 * kBalW) {
-        float s = ps[0][e];
+    float s = 0.0f;
+    const int e = tid;
+    if (e < A.E) {
+        s = ps[0][e];
 #pragma unroll
         for (int w = 1; w < kBalW; w++) s += ps[w][e];
-        po[e] = s;
+    }
+    if (gridDim.x > 1) {
+        if (e <= A.E) A.part[(size_t)blockIdx.x * (A.E + 1) + e] = make_float2(s, __int_as_float(cnt[e]));
+        return;
+    }
+    __syncthreads();
+    if (e < A.E) {
+        A.psum[e] = s;
         ps[0][e] = s;
     }
-    for (int e = tid; e <= A.E; e += 64 * kBalW) co[e] = cnt[e];
-    if (all) {
-        __syncthreads();
-        balance_of(A, cnt, ps[0], red);
-    }
+    if (e <= A.E) A.counts[e] = cnt[e];
+    __syncthreads();
+    balance_of(A, cnt, ps[0]);
 }
 
 // The workgroups' parts to counts, sums and loss: thread (group of parts, expert).
+constexpr int kBalGroups = 128;   // most parts
 __global__ __launch_bounds__(1024) void k_balance_join(BalanceArgs A, int nb) {
-    __shared__ float ps[4][kMaxE];
+    __shared__ float ps[4][kMaxE + 1];
     __shared__ int32_t cs[4][kMaxE + 1];
-    __shared__ double red[64];
-    const int e = threadIdx.x & 255, g = threadIdx.x >> 8;
-    const int32_t *cpart = reinterpret_cast<const int32_t *>(A.part + (size_t)nb * A.E);
-    if (e < A.E) {
+    const int n = A.E + 1;
+    auto add = [&](int e, int g) {
         float s = 0.0f;
         int32_t c = 0;
-#pragma unroll 8
+#pragma unroll 16
         for (int b = g; b < nb; b += 4) {
-            s += A.part[(size_t)b * A.E + e];
-            c += cpart[(size_t)b * (A.E + 1) + e];
+            const float2 v = A.part[(size_t)b * n + e];
+            s += v.x;
+            c += __float_as_int(v.y);
         }
         ps[g][e] = s;
         cs[g][e] = c;
-    }
-    if (e == 0) {
-        int32_t c = 0;
-        for (int b = g; b < nb; b += 4) c += cpart[(size_t)b * (A.E + 1) + A.E];
-        cs[g][A.E] = c;
-    }
+    };
+    const int e = threadIdx.x & 255, g = threadIdx.x >> 8;
+    if (e < n) add(e, g);
+    if (n == 257 && e == 0) add(256, g);
     __syncthreads();
-    for (int i = threadIdx.x; i <= A.E; i += 1024) {
+    for (int i = threadIdx.x; i < n; i += 1024) {
         const int32_t c = cs[0][i] + cs[1][i] + cs[2][i] + cs[3][i];
         cs[0][i] = c;
         A.counts[i] = c;
@@ -179,15 +250,15 @@ __global__ __launch_bounds__(1024) void k_balance_join(BalanceArgs A, int nb) {
         }
     }
     __syncthreads();
-    balance_of(A, cs[0], ps[0], red);
+    balance_of(A, cs[0], ps[0]);
 }
 
-// Workgroups: one up to 256 tokens (no second launch), then 128 tokens each up
-// to 128 of them, whose parts one workgroup still joins in a few microseconds.
+// Workgroups: one up to 128 tokens (no second launch), then 64 tokens each up to
+// kBalGroups of them, whose parts one workgroup still joins in a few microseconds.
 int balance_groups(int T) {
-    if (T <= 256) return 1;
-    const int n = (int)(((int64_t)T + 127) / 128);
-    return n < 128 ? n : 128;
+    if (T <= 128) return 1;
+    const int n = (int)(((int64_t)T + 63) / 64);
+    return n < kBalGroups ? n : kBalGroups;
 }
 
 // ---------------------------------------------------------------------------
@@ -205,86 +276,99 @@ struct LogitGradArgs {
     float scale, coef;
 };
 
-// 16 lanes per token.  The softmax over all experts is formed only where the
-// balance loss or weights that are not renormalised ask for it; the gradients
-// of the picks are added to their experts by the lanes that hold them, in slot
-// order, so an expert that was picked twice gets both.
-template <int NI>
+// 16 lanes per token, 16 tokens per workgroup.  FULL: the softmax over all
+// experts, for the balance loss or for weights that are not renormalised; without
+// it a token's logits are read at its picks alone.  Lane s < k forms the gradient
+// of pick s and puts it into the token's row in LDS, from where the lanes that
+// hold its expert take it; where an expert stands twice the picks are added one
+// after the other instead, in slot order.
+template <int NV, bool FULL>
 __global__ __launch_bounds__(256) void k_logit_grad(LogitGradArgs A) {
-    const int l = threadIdx.x & 15;
-    float f[NI];
+    constexpr int LDS = 64 * NV + 16;   // floats per row: the four tokens of a wave 16 banks apart
+    __shared__ __align__(16) float up_row[16][LDS];
+    const int l = threadIdx.x & 15, slot = threadIdx.x >> 4;
+    const bool balance = FULL && A.counts;
+    float f[NV][4];
     float gain = 0.0f;
-    if (A.counts) {
+    if (balance) {
         const float n = (float)A.counts[A.E];
-        const float den = n * (float)A.k;
+        const float inv = n > 0.0f ? 1.0f / (n * (float)A.k) : 0.0f;
         gain = n > 0.0f ? A.coef * (float)A.E / n * (A.dloss ? *A.dloss : 1.0f) : 0.0f;
 #pragma unroll
-        for (int i = 0; i < NI; i++) f[i] = l + 16 * i < A.E && n > 0.0f ? (float)A.counts[l + 16 * i] / den : 0.0f;
+        for (int i = 0; i < NV; i++)
+#pragma unroll
+            for (int c = 0; c < 4; c++) f[i][c] = (float)A.counts[min(64 * i + 4 * l + c, A.E - 1)] * inv;
     }
-    const bool full = A.counts || (A.dwt && !A.renorm);
-    for (int64_t t = (int64_t)blockIdx.x * 16 + (threadIdx.x >> 4); t < A.T; t += (int64_t)gridDim.x * 16) {
-        float o[NI];
-#pragma unroll
-        for (int i = 0; i < NI; i++) o[i] = 0.0f;
-        if (!A.mask || A.mask[t]) {
-            const float *row = A.logits + (size_t)t * A.ld;
-            float p[NI];
-            if (full) {
-                load_logits(row, A.E, l, p);
-                softmax16(p);
+    for (int64_t t = (int64_t)blockIdx.x * 16 + slot; t < A.T; t += (int64_t)gridDim.x * 16) {
+        const float *row = A.logits + (size_t)t * A.ld;
+        const bool live = !A.mask || A.mask[t];
+        float p[NV][4], u[NV][4];
+        int e = -1;
+        float up = 0.0f, lp = -INFINITY;
+        if (A.dwt && l < A.k) {
+            e = A.idx[(size_t)t * A.k + l];
+            up = A.dwt[(size_t)t * A.k + l] * A.scale;
+            e = (unsigned)e < (unsigned)A.E ? e : -1;   // an index that names no expert: no pick
+        }
+        if (FULL) load16(row, A.E, l, -INFINITY, p);
+        if (A.dwt) {
+            if (A.renorm && e >= 0) lp = row[e];
+            float s = e >= 0 ? up : 0.0f;
+            if (A.renorm) {
+                float q[1][1] = {{lp}};
+                softmax16(q);
+                const float mean = sum16(q[0][0] * s);   // by all 16 lanes, those without a pick too
+                s = e >= 0 ? q[0][0] * (up - mean) : 0.0f;
             }
-            if (A.counts) {
-                float d = 0.0f;
+            // the same expert at two slots of a token: compared with the lanes
+            // 1..7 to the right in the row
+            bool twice = false;
+#define SAME(N) twice |= __builtin_amdgcn_update_dpp(-2, e, 0x100 + N, 0xf, 0xf, false) == e
+            SAME(1); SAME(2); SAME(3); SAME(4); SAME(5); SAME(6); SAME(7);
+#undef SAME
+            twice = twice && e >= 0;
+            float *mine = up_row[slot];
 #pragma unroll
-                for (int i = 0; i < NI; i++) d = fmaf(p[i], f[i], d);
-                d = sum16(d);
-#pragma unroll
-                for (int i = 0; i < NI; i++) o[i] = gain * p[i] * (f[i] - d);
-            }
-            if (A.dwt) {
-                // lane s < k holds slot s; a slot whose index names no expert is none
-                int e = -1;
-                float up = 0.0f;
-                if (l < A.k) {
-                    e = A.idx[(size_t)t * A.k + l];
-                    e = (unsigned)e < (unsigned)A.E ? e : -1;
-                    up = e >= 0 ? A.dwt[(size_t)t * A.k + l] * A.scale : 0.0f;
-                }
-                float s = up;
-                if (A.renorm) {
-                    float q[1] = {e >= 0 ? row[e] : -INFINITY};
-                    softmax16(q);
-                    s = q[0] * (up - sum16(q[0] * up));
-                    s = e >= 0 ? s : 0.0f;
-                }
-                float u[NI];
-#pragma unroll
-                for (int i = 0; i < NI; i++) u[i] = 0.0f;
-#pragma unroll
+            for (int i = 0; i < NV; i++) *reinterpret_cast<float4 *>(&mine[64 * i + 4 * l]) = make_float4(0.f, 0.f, 0.f, 0.f);
+            wave_sync();
+            if (!__any(twice)) {
+                if (e >= 0) mine[e] = s;
+            } else {
                 for (int j = 0; j < kMaxK; j++) {
-                    if (j < A.k) {
-                        const int ej = __shfl(e, j, 16);
-                        const float sj = __shfl(s, j, 16);
-#pragma unroll
-                        for (int i = 0; i < NI; i++) u[i] += ej == l + 16 * i ? sj : 0.0f;
-                    }
-                }
-                if (A.renorm) {
-#pragma unroll
-                    for (int i = 0; i < NI; i++) o[i] += u[i];
-                } else {
-                    float d = 0.0f;
-#pragma unroll
-                    for (int i = 0; i < NI; i++) d = fmaf(p[i], u[i], d);
-                    d = sum16(d);
-#pragma unroll
-                    for (int i = 0; i < NI; i++) o[i] = fmaf(p[i], u[i] - d, o[i]);
+                    if (l == j && e >= 0) mine[e] += s;
+                    wave_sync();
                 }
             }
+            wave_sync();
+#pragma unroll
+            for (int i = 0; i < NV; i++) {
+                const float4 v = *reinterpret_cast<const float4 *>(&mine[64 * i + 4 * l]);
+                u[i][0] = v.x; u[i][1] = v.y; u[i][2] = v.z; u[i][3] = v.w;
+            }
+            wave_sync();
+        } else {
+#pragma unroll
+            for (int i = 0; i < NV; i++)
+#pragma unroll
+                for (int c = 0; c < 4; c++) u[i][c] = 0.0f;
+        }
+        if (FULL) {
+            softmax16(p);
+            const float d = balance ? dot16(p, f) : 0.0f;
+            const float du = A.dwt && !A.renorm ? dot16(p, u) : 0.0f;
+#pragma unroll
+            for (int i = 0; i < NV; i++)
+#pragma unroll
+                for (int c = 0; c < 4; c++) {
+                    if (!A.renorm) u[i][c] = p[i][c] * (u[i][c] - du);
+                    if (balance) u[i][c] = fmaf(gain * p[i][c], f[i][c] - d, u[i][c]);
+                }
         }
 #pragma unroll
-        for (int i = 0; i < NI; i++)
-            if (l + 16 * i < A.E) A.out[(size_t)t * A.ldo + l + 16 * i] = o[i];
+        for (int i = 0; i < NV; i++)
+#pragma unroll
+            for (int c = 0; c < 4; c++) u[i][c] = live ? u[i][c] : 0.0f;
+        store16(A.out + (size_t)t * A.ldo, A.E, l, u);
     }
 }
 
@@ -294,9 +378,10 @@ __global__ __launch_bounds__(256) void k_logit_grad(LogitGradArgs A) {
 typedef float f32x16 __attribute__((ext_vector_type(16)));
 typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef uint32_t u32x2_t __attribute__((ext_vector_type(2)));
 
 constexpr int kRgD = 2048;
-constexpr int kMaxRouterT = 1 << 25, kMaxRouterRows = 1 << 20;
+constexpr int kMaxRouterT = 1 << 25, kMaxRouterRows = 1 << 20, kMaxRouterLd = 1 << 22;
 
 struct ProductArgs {
     const float *w, *dl, *dsh;   // [n_rows][kRgD]; [T][ld]; the shared gate's column, stride ld_sh
@@ -315,21 +400,18 @@ __device__ __forceinline__ int c_row(int i, int lane) { return 8 * (i >> 2) + 4 
 
 // Workgroup barrier for LDS data only: prefetched global loads stay in flight.
 __device__ __forceinline__ void lds_barrier() { asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
-__device__ __forceinline__ void wave_sync() {
-    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
-    __builtin_amdgcn_wave_barrier();
-    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
-}
 
 // Workgroup b of n in an order in which those of one XCD (b % 8) are neighbours.
 __device__ __forceinline__ int xcd_order(int b, int n) { return (n & 7) ? b : (b & 7) * (n >> 3) + (b >> 3); }
 
 // ---- few tokens: fp32 MFMA ----
 // v_mfma_f32_32x32x2_f32: lane L holds row (A) or column (B) L % 32 at K element
-// L / 32.  One 32 x 32 tile per wave, no LDS: the products cost 64 cycles each,
-// and a wave's operands come straight from the caches, the next batch of loads
-// issued before the products of this one.  dW and dx share the launch.
-constexpr int kF32Batch = 16;
+// L / 32.  One tile of 32 rows x 64 columns per workgroup, whose four waves take a
+// quarter of K each and add up through LDS: at these sizes a tile's time is the
+// round trips of its loads (203 tokens, a wave per 32 x 32 tile and all of K: dW
+// 10.6, dx 9.4 us).  Operands come straight from the caches in batches, the next
+// batch's loads ahead of the products of this one.  dW and dx share the launch.
+constexpr int kF32Cols = 64;
 
 template <int XF>
 __device__ __forceinline__ float load_x(const void *x, size_t at) {
@@ -337,113 +419,142 @@ __device__ __forceinline__ float load_x(const void *x, size_t at) {
     else return __uint_as_float((uint32_t)static_cast<const uint16_t *>(x)[at] << 16);
 }
 
+struct Tile2 { f32x16 c[2]; };   // columns L % 32 and 32 + L % 32
+
+__device__ __forceinline__ void mfma2(Tile2 &t, float a, float b0, float b1) {
+    t.c[0] = __builtin_amdgcn_mfma_f32_32x32x2f32(a, b0, t.c[0], 0, 0, 0);
+    t.c[1] = __builtin_amdgcn_mfma_f32_32x32x2f32(a, b1, t.c[1], 0, 0, 0);
+}
+
+// A quarter of the tokens: dlogits^T x.  Batches of 16 K-steps; tokens past the
+// end read the last one and count as zeros.
 template <int XF>
-__device__ __forceinline__ void f32_dw_tile(const ProductArgs &A, int rt, int d0) {
-    constexpr int U = kF32Batch;
-    const int lane = threadIdx.x & 63, half = lane >> 5, c = lane & 31;
-    const int r = min(rt * 32 + c, A.n_rows - 1);
-    const bool sh = r >= A.n_expert;
-    const float *col = sh ? A.dsh : A.dl + r;
-    const int64_t step = sh ? A.ld_sh : A.ld;
-    f32x16 acc = {};
-    float a[2][U], b[2][U];
-    auto load = [&](int t, float (&av)[U], float (&bv)[U]) {
+__device__ __forceinline__ Tile2 f32_dw_dot(const ProductArgs &A, int wave, int half, const float *col, int64_t step, int d) {
+    constexpr int U = 16;
+    Tile2 acc = {};
+    const int quarter = ((A.T + 7) >> 3) << 1, t0 = wave * quarter, t1 = min(t0 + quarter, A.T);
+    float a[2][U], b[2][U][2];
+    auto load = [&](int t, float (&av)[U], float (&bv)[U][2]) {
 #pragma unroll
         for (int u = 0; u < U; u++) {
-            const int tc = min(t + 2 * u + half, A.T - 1);
+            const int tc = min(t + 2 * u + half, t1 - 1);
             av[u] = col[tc * step];
-            bv[u] = load_x<XF>(A.x, (size_t)tc * kRgD + d0 + c);
+            bv[u][0] = load_x<XF>(A.x, (size_t)tc * kRgD + d);
+            bv[u][1] = load_x<XF>(A.x, (size_t)tc * kRgD + d + 32);
         }
     };
-    auto products = [&](int t, const float (&av)[U], const float (&bv)[U]) {
+    auto products = [&](int t, const float (&av)[U], const float (&bv)[U][2]) {
 #pragma unroll
         for (int u = 0; u < U; u++) {
-            const bool in = t + 2 * u + half < A.T;   // past the end the last token again, as zeros
-            acc = __builtin_amdgcn_mfma_f32_32x32x2f32(in ? av[u] : 0.0f, in ? bv[u] : 0.0f, acc, 0, 0, 0);
+            const bool in = t + 2 * u + half < t1;
+            mfma2(acc, in ? av[u] : 0.0f, in ? bv[u][0] : 0.0f, in ? bv[u][1] : 0.0f);
         }
     };
-    load(0, a[0], b[0]);
-    for (int t = 0; t < A.T; t += 4 * U) {
-        if (t + 2 * U < A.T) load(t + 2 * U, a[1], b[1]);
+    if (t0 >= t1) return acc;
+    load(t0, a[0], b[0]);
+    for (int t = t0; t < t1; t += 4 * U) {
+        if (t + 2 * U < t1) load(t + 2 * U, a[1], b[1]);
         products(t, a[0], b[0]);
-        if (t + 2 * U < A.T) {
-            if (t + 4 * U < A.T) load(t + 4 * U, a[0], b[0]);
+        if (t + 2 * U < t1) {
+            if (t + 4 * U < t1) load(t + 4 * U, a[0], b[0]);
             products(t + 2 * U, a[1], b[1]);
         }
     }
-#pragma unroll
-    for (int i = 0; i < 16; i++) {
-        const int row = rt * 32 + c_row(i, lane);
-        if (row < A.n_rows) A.dw[(size_t)row * kRgD + d0 + c] = acc[i];
-    }
+    return acc;
 }
 
-// Lane half h of a step of 8 rows holds rows 4h..4h+3 of both operands.
-template <int XF>
-__device__ __forceinline__ void f32_dx_tile(const ProductArgs &A, int tb, int d0) {
-    constexpr int U = kF32Batch / 4;
-    const int lane = threadIdx.x & 63, half = lane >> 5, c = lane & 31;
-    const int t = min(tb + c, A.T - 1);
-    const float *row = A.dl + (size_t)t * A.ld, *col = A.w + d0 + c;
-    f32x16 acc = {};
-    float a[2][U][4], b[2][U][4];
-    auto load = [&](int r0, float (&av)[U][4], float (&bv)[U][4]) {
+// A quarter of a token's router rows: dlogits W.  The rows are neighbours in
+// memory, so a lane takes four at a time (half h of a step of 8 holds rows
+// 4 h..4 h + 3 of both operands; one row per load, with 64 lanes in 32 tokens'
+// rows, nearly doubled the time).  The rows past the last whole step, the shared
+// gate's among them, go to the last wave.
+__device__ __forceinline__ Tile2 f32_dx_dot(const ProductArgs &A, int wave, int half, const float *row, const float *gate,
+                                            const float *col) {
+    constexpr int U = 4;
+    Tile2 acc = {};
+    float a[2][U][4], b[2][U][4][2];
+    const int whole = A.n_expert & ~7, quarter = ((whole >> 3) + 3) / 4 * 8;
+    const int k0 = wave * quarter, k1 = min(k0 + quarter, whole);
+    auto load = [&](int k, float (&av)[U][4], float (&bv)[U][4][2]) {
 #pragma unroll
         for (int u = 0; u < U; u++) {
-            const int r = r0 + 8 * u + 4 * half;
+            const int r = min(k + 8 * u, k1 - 8) + 4 * half;   // past the end the last step again
             load_row<Q36MOE_FMT_F32>(row, r, av[u]);
 #pragma unroll
-            for (int i = 0; i < 4; i++) bv[u][i] = col[(size_t)(r + i) * kRgD];
+            for (int i = 0; i < 4; i++) {
+                bv[u][i][0] = col[(size_t)(r + i) * kRgD];
+                bv[u][i][1] = col[(size_t)(r + i) * kRgD + 32];
+            }
         }
     };
-    auto products = [&](const float (&av)[U][4], const float (&bv)[U][4]) {
+    auto products = [&](int k, const float (&av)[U][4], const float (&bv)[U][4][2]) {
 #pragma unroll
         for (int u = 0; u < U; u++)
+            if (k + 8 * u < k1)
 #pragma unroll
-            for (int i = 0; i < 4; i++) acc = __builtin_amdgcn_mfma_f32_32x32x2f32(av[u][i], bv[u][i], acc, 0, 0, 0);
+                for (int i = 0; i < 4; i++) mfma2(acc, av[u][i], bv[u][i][0], bv[u][i][1]);
     };
-    const int whole = A.n_expert & ~(8 * U - 1);
-    if (whole) load(0, a[0], b[0]);
-    for (int r0 = 0; r0 < whole; r0 += 16 * U) {
-        if (r0 + 8 * U < whole) load(r0 + 8 * U, a[1], b[1]);
-        products(a[0], b[0]);
-        if (r0 + 8 * U < whole) {
-            if (r0 + 16 * U < whole) load(r0 + 16 * U, a[0], b[0]);
-            products(a[1], b[1]);
+    if (k0 < k1) {
+        load(k0, a[0], b[0]);
+        for (int k = k0; k < k1; k += 16 * U) {
+            if (k + 8 * U < k1) load(k + 8 * U, a[1], b[1]);
+            products(k, a[0], b[0]);
+            if (k + 8 * U < k1) {
+                if (k + 16 * U < k1) load(k + 16 * U, a[0], b[0]);
+                products(k + 8 * U, a[1], b[1]);
+            }
         }
     }
-    // the rows left over, the shared gate's among them
-    for (int r0 = whole; r0 < A.n_rows; r0 += 16) {
-        float av[8], bv[8];
+    if (wave == 3 && whole < A.n_rows) {
+        float av[4], b0[4], b1[4];
 #pragma unroll
-        for (int u = 0; u < 8; u++) {
-            const int r = min(r0 + 2 * u + half, A.n_rows - 1);
-            av[u] = r < A.n_expert ? row[r] : A.dsh[(size_t)t * A.ld_sh];
-            bv[u] = col[(size_t)r * kRgD];
+        for (int u = 0; u < 4; u++) {
+            const int r = min(whole + 2 * u + half, A.n_rows - 1);
+            av[u] = r < A.n_expert ? row[r] : *gate;
+            b0[u] = col[(size_t)r * kRgD];
+            b1[u] = col[(size_t)r * kRgD + 32];
         }
 #pragma unroll
-        for (int u = 0; u < 8; u++) {
-            const bool in = r0 + 2 * u + half < A.n_rows;
-            acc = __builtin_amdgcn_mfma_f32_32x32x2f32(in ? av[u] : 0.0f, in ? bv[u] : 0.0f, acc, 0, 0, 0);
+        for (int u = 0; u < 4; u++) {
+            const bool in = whole + 2 * u + half < A.n_rows;
+            mfma2(acc, in ? av[u] : 0.0f, in ? b0[u] : 0.0f, in ? b1[u] : 0.0f);
         }
     }
-#pragma unroll
-    for (int i = 0; i < 16; i++) {
-        const int tt = tb + c_row(i, lane);
-        if (tt < A.T) store_one<XF>(A.dx, (size_t)tt * kRgD + d0 + c, acc[i]);
-    }
+    return acc;
 }
-
-constexpr int kF32Cols = 128;   // columns per workgroup, 32 per wave
 
 template <int XF>
 __global__ __launch_bounds__(256) void k_router_grad_f32(ProductArgs A) {
-    const int wave = threadIdx.x >> 6;
+    __shared__ float red[4][32][64];
+    const int lane = threadIdx.x & 63, half = lane >> 5, c = lane & 31;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const bool is_dw = (int)blockIdx.x < A.nw;
     const int b = is_dw ? blockIdx.x : blockIdx.x - A.nw;
-    const int d0 = b % (kRgD / kF32Cols) * kF32Cols + wave * 32, tile = b / (kRgD / kF32Cols);
-    if (is_dw) f32_dw_tile<XF>(A, tile, d0);
-    else f32_dx_tile<XF>(A, tile * 32, d0);
+    const int d = b % (kRgD / kF32Cols) * kF32Cols + c, m0 = b / (kRgD / kF32Cols) * 32;
+    Tile2 acc;
+    if (is_dw) {
+        const int r = min(m0 + c, A.n_rows - 1);
+        const bool sh = r >= A.n_expert;
+        acc = f32_dw_dot<XF>(A, wave, half, sh ? A.dsh : A.dl + r, sh ? A.ld_sh : A.ld, d);
+    } else {
+        const int t = min(m0 + c, A.T - 1);
+        acc = f32_dx_dot(A, wave, half, A.dl + (size_t)t * A.ld, A.dsh + (int64_t)t * A.ld_sh, A.w + d);
+    }
+#pragma unroll
+    for (int j = 0; j < 2; j++)
+#pragma unroll
+        for (int i = 0; i < 16; i++) red[wave][16 * j + i][lane] = acc.c[j][i];
+    __syncthreads();
+#pragma unroll
+    for (int q = 0; q < 8; q++) {
+        const int i = 8 * wave + q, m = m0 + c_row(i & 15, lane), col = d + 32 * (i >> 4);
+        const float v = (red[0][i][lane] + red[1][i][lane]) + (red[2][i][lane] + red[3][i][lane]);
+        if (is_dw) {
+            if (m < A.n_rows) A.dw[(size_t)m * kRgD + col] = v;
+        } else if (m < A.T) {
+            store_one<XF>(A.dx, (size_t)m * kRgD + col, v);
+        }
+    }
 }
 
 // ---- dW of many tokens: operands split into bf16 ----
@@ -499,8 +610,10 @@ __global__ __launch_bounds__(512) void k_router_dw_split(ProductArgs A) {
     const int r0 = (mb * MW + wm) * 32;
     const int t0 = split * A.span, t1 = min(t0 + A.span, A.T);
     const bool gate = A.n_rows > A.n_expert && mb == 0;
-    const float *dl = A.dl + min(r0 + c, A.n_expert - 1);
-
+    // the shared gate's gradients, or any others where no row of it is formed
+    // (its sums are then not stored): no condition in the loop
+    const float *gcol = gate ? A.dsh : A.dl;
+    const int64_t gstep = gate ? A.ld_sh : A.ld;
     f32x16 acc[NT];
 #pragma unroll
     for (int j = 0; j < NT; j++) acc[j] = f32x16{};
@@ -509,68 +622,113 @@ __global__ __launch_bounds__(512) void k_router_dw_split(ProductArgs A) {
     uint32_t xr[8][F32 ? 2 : 1];              // tokens t + 8 wave + i, columns n0 + 2 lane, + 1
     float sh[8];
 
-    auto load = [&](int t, float (&av)[4][8]) {
+    // Whole steps load through buffers based at the step's first row, with the
+    // rows as scalar offsets: no address arithmetic on the vector unit.  In the
+    // split's last step tokens past its end are zeros.
+    const int lr = min(r0 + c, A.n_expert - 1);
+    const uint32_t lo = (uint32_t)(8 * half * A.ld + lr) * 4u;
+    auto load_x = [&](int t, auto WHOLE) {
         const int tx = t + 8 * wave;
-#pragma unroll
-        for (int i = 0; i < 8; i++) {
-            const size_t o = (size_t)min(tx + i, A.T - 1) * kRgD + n0 + 2 * lane;
+        if (decltype(WHOLE)::value || t + kDwStep <= t1) {
+            const size_t at = (size_t)tx * kRgD + n0;
             if constexpr (F32) {
-                const float2 v = *reinterpret_cast<const float2 *>(static_cast<const float *>(A.x) + o);
-                xr[i][0] = __float_as_uint(v.x);
-                xr[i][1] = __float_as_uint(v.y);
+                const __amdgpu_buffer_rsrc_t r = __builtin_amdgcn_make_buffer_rsrc(
+                    const_cast<float *>(static_cast<const float *>(A.x) + at), (short)0, 0x7ffffffe, 0x00020000);
+#pragma unroll
+                for (int i = 0; i < 8; i++) {
+                    const auto v = __builtin_amdgcn_raw_buffer_load_b64(r, lane * 8, i * kRgD * 4, 0);
+                    xr[i][0] = v[0];
+                    xr[i][1] = v[1];
+                }
             } else {
-                xr[i][0] = *reinterpret_cast<const uint32_t *>(static_cast<const uint16_t *>(A.x) + o);
+                const __amdgpu_buffer_rsrc_t r = __builtin_amdgcn_make_buffer_rsrc(
+                    const_cast<uint16_t *>(static_cast<const uint16_t *>(A.x) + at), (short)0, 0x7ffffffe, 0x00020000);
+#pragma unroll
+                for (int i = 0; i < 8; i++) xr[i][0] = __builtin_amdgcn_raw_buffer_load_b32(r, lane * 4, i * kRgD * 2, 0);
+            }
+#pragma unroll
+            for (int i = 0; i < 8; i++) sh[i] = gcol[(tx + i) * gstep];
+        } else {
+#pragma unroll
+            for (int i = 0; i < 8; i++) {
+                const int tc = min(tx + i, t1 - 1);
+                const size_t at = (size_t)tc * kRgD + n0 + 2 * lane;
+                uint32_t v0, v1 = 0;
+                if constexpr (F32) {
+                    v0 = static_cast<const uint32_t *>(A.x)[at];
+                    v1 = static_cast<const uint32_t *>(A.x)[at + 1];
+                } else {
+                    v0 = *reinterpret_cast<const uint32_t *>(static_cast<const uint16_t *>(A.x) + at);
+                }
+                xr[i][0] = tx + i < t1 ? v0 : 0u;
+                if constexpr (F32) xr[i][1] = tx + i < t1 ? v1 : 0u;
+                const float v = gcol[tc * gstep];
+                sh[i] = tx + i < t1 ? v : 0.0f;
             }
         }
-        if (gate)
-#pragma unroll
-            for (int i = 0; i < 8; i++) sh[i] = A.dsh[(int64_t)min(tx + i, A.T - 1) * A.ld_sh];
-#pragma unroll
-        for (int k = 0; k < 4; k++)
-#pragma unroll
-            for (int i = 0; i < 8; i++) av[k][i] = dl[(int64_t)min(t + 16 * k + 8 * half + i, A.T - 1) * A.ld];
     };
-    // this step's x to LDS; tokens past the split's end count as zeros
-    auto convert = [&](int t, int buf) {
-        const int left = t1 - (t + 8 * wave);
-        if (left < 8)
+    auto load_a = [&](int t, float (&av)[4][8], auto WHOLE) {
+        if (decltype(WHOLE)::value || t + kDwStep <= t1) {
+            const __amdgpu_buffer_rsrc_t r = __builtin_amdgcn_make_buffer_rsrc(const_cast<float *>(A.dl + (size_t)t * A.ld), (short)0,
+                                                                               0x7ffffffe, 0x00020000);
 #pragma unroll
-            for (int i = 0; i < 8; i++)
+            for (int k = 0; k < 4; k++)
 #pragma unroll
-                for (int u = 0; u < (F32 ? 2 : 1); u++) xr[i][u] = i < left ? xr[i][u] : 0u;
+                for (int i = 0; i < 8; i++)
+                    av[k][i] = __uint_as_float(__builtin_amdgcn_raw_buffer_load_b32(r, lo, (16 * k + i) * A.ld * 4, 0));
+        } else {
+#pragma unroll
+            for (int k = 0; k < 4; k++)
+#pragma unroll
+                for (int i = 0; i < 8; i++) {
+                    const int tt = t + 16 * k + 8 * half + i;
+                    const float v = A.dl[(size_t)min(tt, t1 - 1) * A.ld + lr];
+                    av[k][i] = tt < t1 ? v : 0.0f;
+                }
+        }
+    };
+    auto convert = [&](int buf) {             // this wave's tokens of x to LDS
         const int k = wave >> 1, at = (lane & 31) + 32 * (wave & 1), q = lane >> 5;
 #pragma unroll
         for (int u = 0; u < 2; u++) {
-            if constexpr (F32) {
-                float v[8];
+            float v[8];
 #pragma unroll
-                for (int i = 0; i < 8; i++) v[i] = __uint_as_float(xr[i][u]);
+            for (int i = 0; i < 8; i++)
+                v[i] = F32 ? __uint_as_float(xr[i][F32 ? u : 0]) : u ? bf16_hi(xr[i][0]) : bf16_lo(xr[i][0]);
+            if constexpr (F32) {
                 const Pieces s = split3(v);
 #pragma unroll
                 for (int p = 0; p < NP; p++) sx[buf][p][k][2 * q + u][at] = s.p[p];
-                if (gate)
-#pragma unroll
-                    for (int i = 0; i < 8; i++) sg[u] = fmaf(i < left ? sh[i] : 0.0f, v[i], sg[u]);
             } else {
                 u32x4_u h;
 #pragma unroll
                 for (int i = 0; i < 4; i++)   // the columns' halves of two tokens side by side
                     h[i] = __builtin_amdgcn_perm(xr[2 * i + 1][0], xr[2 * i][0], u ? 0x07060302u : 0x05040100u);
                 sx[buf][0][k][2 * q + u][at] = __builtin_bit_cast(bf16x8, h);
-                if (gate)
-#pragma unroll
-                    for (int i = 0; i < 8; i++)
-                        sg[u] = fmaf(i < left ? sh[i] : 0.0f, u ? bf16_hi(xr[i][0]) : bf16_lo(xr[i][0]), sg[u]);
             }
+#pragma unroll
+            for (int i = 0; i < 8; i++) sg[u] = fmaf(sh[i], v[i], sg[u]);
         }
     };
-    auto products = [&](int t, int buf, float (&av)[4][8]) {
+    // One step: the products of its 64 tokens from LDS, and beside them, in the
+    // 32 cycles that each MFMA runs, the split of the next 16 tokens' gradients,
+    // the conversion of the next step's x into the other buffer and the loads of
+    // the step after it.  One barrier: a step's x is in LDS before it, and every
+    // wave has read the buffer that is written after it.  The steady steps have
+    // no conditions, which keeps them one block for the scheduler and the waits
+    // before a use counted (after a load that may not have been made they are for
+    // every load).
+    Pieces s;                                 // of this step's first 16 tokens
+    auto step = [&](int t, int buf, float (&av)[4][8], const float (&an)[4][8], auto STEADY) {
+        constexpr bool ST = decltype(STEADY)::value;
+        constexpr int NM = NP == 3 ? 6 : 3;   // products per tile
+        const bool one = ST || t + kDwStep < t1, two = ST || t + 2 * kDwStep < t1;
+        lds_barrier();
 #pragma unroll
         for (int k = 0; k < 4; k++) {
-            if (t + 64 > t1)
-#pragma unroll
-                for (int i = 0; i < 8; i++) av[k][i] = t + 16 * k + 8 * half + i < t1 ? av[k][i] : 0.0f;
-            const Pieces s = split3(av[k]);
+            const Pieces next = split3(k < 3 ? av[k < 3 ? k + 1 : 0] : an[0]);
+            if (k == 0 && one) convert(buf ^ 1);
+            if (k == 1 && two) load_x(t + 2 * kDwStep, STEADY);
 #pragma unroll
             for (int j = 0; j < NT; j++) {
                 bf16x8 x[NP];
@@ -583,20 +741,44 @@ __global__ __launch_bounds__(512) void k_router_dw_split(ProductArgs A) {
                     for (int p = 0; p <= o; p++)
                         if (p < NP) acc[j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(s.p[o - p], x[p], acc[j], 0, 0, 0);
             }
+            s = next;
+        }
+        if (two) load_a(t + 2 * kDwStep, av, STEADY);
+        // LDS reads of a tile, then its MFMAs with vector instructions between
+        // (masks: 0x100 LDS read, 0x8 MFMA, 0x2 vector)
+        constexpr int V = (4 * 44 + (F32 ? 104 : 40) + 4 * NT * NM - 1) / (4 * NT * NM);
+#pragma unroll
+        for (int k = 0; k < 4 * NT; k++) {
+            if (k == 0) __builtin_amdgcn_sched_group_barrier(0x100, NP, 0);   // one tile ahead
+            __builtin_amdgcn_sched_group_barrier(0x100, NP, 0);
+#pragma unroll
+            for (int m = 0; m < NM; m++) {
+                __builtin_amdgcn_sched_group_barrier(0x8, 1, 0);
+                __builtin_amdgcn_sched_group_barrier(0x2, V, 0);
+            }
         }
     };
-    load(t0, a[0]);
-    for (int t = t0; t < t1; t += 2 * kDwStep) {
-        convert(t, 0);
-        if (t + kDwStep < t1) load(t + kDwStep, a[1]);
-        lds_barrier();
-        products(t, 0, a[0]);
-        if (t + kDwStep < t1) {
-            convert(t + kDwStep, 1);
-            if (t + 2 * kDwStep < t1) load(t + 2 * kDwStep, a[0]);
-            lds_barrier();
-            products(t + kDwStep, 1, a[1]);
-        }
+    load_x(t0, std::false_type{});
+    load_a(t0, a[0], std::false_type{});
+    convert(0);
+    if (t0 + kDwStep < t1) {
+        load_x(t0 + kDwStep, std::false_type{});
+        load_a(t0 + kDwStep, a[1], std::false_type{});
+    } else {
+#pragma unroll
+        for (int i = 0; i < 32; i++) a[1][i >> 3][i & 7] = 0.0f;
+    }
+    s = split3(a[0][0]);
+    int t = t0;
+#pragma unroll 1
+    for (; t + 4 * kDwStep <= t1; t += 2 * kDwStep) {
+        step(t, 0, a[0], a[1], std::true_type{});
+        step(t + kDwStep, 1, a[1], a[0], std::true_type{});
+    }
+#pragma unroll 1
+    for (; t < t1; t += 2 * kDwStep) {
+        step(t, 0, a[0], a[1], std::false_type{});
+        if (t + kDwStep < t1) step(t + kDwStep, 1, a[1], a[0], std::false_type{});
     }
     float *o = A.dw + (size_t)split * A.n_rows * kRgD;
 #pragma unroll
@@ -631,7 +813,9 @@ __global__ __launch_bounds__(512) void k_router_dw_split(ProductArgs A) {
 // can be scaled by a power of two that puts the largest at 2^14..2^15: two f16
 // (11 bits each) then hold a value to 2^-22 of itself, or to 2^-40 of the
 // largest where that is more, and three products of v_mfma_f32_32x32x16_f16
-// give fp32's exactness (the fourth is 2^-22 of the first).
+// give fp32's exactness (the fourth is 2^-22 of the first).  The same for a bf16
+// dx: one f16 per operand would be a third of the products, but 2^-10 of each
+// term, which is above the result's own rounding where the terms cancel.
 // Workgroup: 256 tokens, 32 per wave with their gradients in registers, against
 // its part of the columns, 64 at a time through LDS.
 __device__ __forceinline__ int scale_exp(float amax) {   // amax * 2^this is in [2^14, 2^15)
@@ -639,12 +823,13 @@ __device__ __forceinline__ int scale_exp(float amax) {   // amax * 2^this is in 
     return 141 - max(e, 1);
 }
 
-__device__ __forceinline__ void split_f16(const float (&v)[8], int e, f16x8 (&p)[2]) {
+template <int NP>
+__device__ __forceinline__ void split_f16(const float (&v)[8], int e, f16x8 (&p)[NP]) {
 #pragma unroll
     for (int i = 0; i < 8; i++) {
         const float s = __builtin_ldexpf(v[i], e);
         p[0][i] = (_Float16)s;
-        p[1][i] = (_Float16)(s - (float)p[0][i]);
+        if constexpr (NP > 1) p[1][i] = (_Float16)(s - (float)p[0][i]);
     }
 }
 
@@ -652,10 +837,11 @@ constexpr int kDxRows = 256, kDxCols = 64, kDxStages = kRgD / kDxCols;
 
 template <int XF, int KS>   // K-steps of 16: 8 or 16
 __global__ __launch_bounds__(512) void k_router_dx_split(ProductArgs A) {
+    constexpr int NP = 2;                     // pieces of an operand
     constexpr int JW = KS / 8;                // K-steps of W that a wave converts
     constexpr int LDA = 68;                   // floats per staged row of 64: rows 4 banks apart
     __shared__ __align__(16) float sa[8][32 * LDA];
-    __shared__ __align__(16) f16x8 sw[2][2][KS][64];
+    __shared__ __align__(16) f16x8 sw[NP][2][KS][64];
     __shared__ __align__(16) float cmax[8][kDxCols];
     __shared__ __align__(16) int srow[8][32];
     __shared__ __align__(16) float sgate[8][32];
@@ -671,6 +857,12 @@ __global__ __launch_bounds__(512) void k_router_dx_split(ProductArgs A) {
     // W through a buffer that ends with the last expert's row: rows past it
     // read as zeros
     const __amdgpu_buffer_rsrc_t rw = __builtin_amdgcn_make_buffer_rsrc(const_cast<float *>(A.w), (short)0, E * kRgD * 4, 0x00020000);
+    // dx through one that ends with the last token's row: rows past it are not
+    // stored, without a branch around a store (which would make the next wait for
+    // W one for every store as well)
+    constexpr int XB = XF == Q36MOE_FMT_F32 ? 4 : 2;
+    const __amdgpu_buffer_rsrc_t rdx = __builtin_amdgcn_make_buffer_rsrc(
+        static_cast<uint8_t *>(A.dx) + (size_t)min(tw, A.T - 1) * kRgD * XB, (short)0, max(min(A.T - tw, 32), 0) * kRgD * XB, 0x00020000);
     float2 wr[JW][8];
     auto load_w = [&](int st) {
 #pragma unroll
@@ -686,7 +878,7 @@ __global__ __launch_bounds__(512) void k_router_dx_split(ProductArgs A) {
 
     // the wave's gradients to operand order, 64 columns at a time through its
     // own LDS; columns past the last expert are zeros
-    f16x8 ga[KS][2];
+    f16x8 ga[KS][NP];
     {
         float4 g[2][8];   // two groups of 64 columns in flight
         auto load_g = [&](int p, float4 (&v4)[8]) {
@@ -732,7 +924,7 @@ __global__ __launch_bounds__(512) void k_router_dx_split(ProductArgs A) {
         const int e = scale_exp(fmaxf(m, __shfl_xor(m, 32, 64)));
         if (lane < 32) srow[wave][lane] = -e;
 #pragma unroll
-        for (int k = 0; k < KS; k++) split_f16(raw[k], e, ga[k]);
+        for (int k = 0; k < KS; k++) split_f16<NP>(raw[k], e, ga[k]);
     }
     for (int st = s0; st < s1; st++) {
         const int n0 = st * kDxCols;
@@ -758,17 +950,17 @@ __global__ __launch_bounds__(512) void k_router_dx_split(ProductArgs A) {
 #pragma unroll
         for (int j = 0; j < JW; j++) {
             float v[8];
-            f16x8 h[2];
+            f16x8 h[NP];
 #pragma unroll
             for (int i = 0; i < 8; i++) v[i] = wr[j][i].x;
-            split_f16(v, e0, h);
+            split_f16<NP>(v, e0, h);
 #pragma unroll
-            for (int p = 0; p < 2; p++) sw[p][0][wave * JW + j][lane] = h[p];
+            for (int p = 0; p < NP; p++) sw[p][0][wave * JW + j][lane] = h[p];
 #pragma unroll
             for (int i = 0; i < 8; i++) v[i] = wr[j][i].y;
-            split_f16(v, e1, h);
+            split_f16<NP>(v, e1, h);
 #pragma unroll
-            for (int p = 0; p < 2; p++) sw[p][1][wave * JW + j][lane] = h[p];
+            for (int p = 0; p < NP; p++) sw[p][1][wave * JW + j][lane] = h[p];
         }
         if (st + 1 < s1) load_w(st + 1);
         float2 wg = make_float2(0.0f, 0.0f);
@@ -786,21 +978,26 @@ __global__ __launch_bounds__(512) void k_router_dx_split(ProductArgs A) {
             }
 #pragma unroll
         for (int i = 0; i < 16; i++) {
-            const int r = c_row(i, lane), t = tw + r;
+            const int r = c_row(i, lane);
             const int er = srow[wave][r];
             const float g = sgate[wave][r];
             const float v0 = fmaf(g, wg.x, __builtin_ldexpf(acc[0][i], er - e0)), v1 = fmaf(g, wg.y, __builtin_ldexpf(acc[1][i], er - e1));
-            if (t < A.T) {
-                const size_t o = (size_t)t * kRgD + n0 + 2 * c;
-                if constexpr (XF == Q36MOE_FMT_F32) *reinterpret_cast<float2 *>(static_cast<float *>(A.dx) + o) = make_float2(v0, v1);
-                else *reinterpret_cast<uint32_t *>(static_cast<uint16_t *>(A.dx) + o) = bf16_pair(v0, v1);
-            }
+            if constexpr (XF == Q36MOE_FMT_F32)
+                __builtin_amdgcn_raw_buffer_store_b64(u32x2_t{__float_as_uint(v0), __float_as_uint(v1)}, rdx, r * kRgD * 4 + 8 * c, n0 * 4, 0);
+            else
+                __builtin_amdgcn_raw_buffer_store_b32(bf16_pair(v0, v1), rdx, r * kRgD * 2 + 4 * c, n0 * 2, 0);
         }
     }
 }
 
 constexpr int kCUs = 256;
-constexpr int kSplitT = 512;      // tokens from which the split operands pay
+
+// Tokens from which the split operands pay.  Their time is nearly flat there (two
+// launches of one workgroup per CU, and the sum of dW's splits), that of the fp32
+// tiles grows with the tokens.  us of both gradients, fp32 x (fp32 tiles / split):
+// 256 + 1 rows, 512 tokens 27 / 32, 700 35 / 33, 1024 46 / 36; 128 rows, 700
+// 19 / 22, 1024 24 / 25, 1400 31 / 27; 60 rows, 1024 20 / 25, 1400 27 / 27, 2048 36 / 29.
+int split_from(int n_expert) { return n_expert > 128 ? 640 : n_expert > 64 ? 1024 : 1400; }
 
 // Waves along the router rows in k_router_dw_split.
 int dw_mw(int n_expert) { return n_expert <= 64 ? 2 : n_expert <= 128 ? 4 : 8; }
@@ -814,7 +1011,7 @@ int dw_span(int T, int n_expert) {
     return span > 2 * kDwStep ? span : 2 * kDwStep;
 }
 int dw_splits(int T, int n_expert) {
-    if (T < kSplitT) return 1;
+    if (T < split_from(n_expert)) return 1;
     const int span = dw_span(T, n_expert);
     return (T + span - 1) / span;
 }
@@ -822,7 +1019,7 @@ int dw_splits(int T, int n_expert) {
 template <int XF>
 void launch_product(const ProductArgs &P, float *dw, float *ws, hipStream_t s) {
     ProductArgs A = P;
-    const bool many = A.T >= kSplitT;
+    const bool many = A.T >= split_from(A.n_expert);
     const bool dw_many = dw && many, dx_many = A.dx && many && A.n_expert <= 256;
     if (dw_many) {
         const int mw = dw_mw(A.n_expert), splits = dw_splits(A.T, A.n_expert);
@@ -857,7 +1054,7 @@ extern "C" {
 size_t q36moe_balance_loss_workspace(int T, int n_expert) {
     if (T < 1 || n_expert < 1 || n_expert > kMaxE) return 0;
     const int nb = balance_groups(T);
-    return nb == 1 ? 0 : (size_t)nb * (2 * n_expert + 1) * sizeof(float);
+    return nb == 1 ? 0 : (size_t)nb * (n_expert + 1) * sizeof(float2);
 }
 
 int q36moe_balance_loss(const float *logits, int ld, const int32_t *idx, const uint8_t *mask, int T, int n_expert, int k,
@@ -867,12 +1064,12 @@ int q36moe_balance_loss(const float *logits, int ld, const int32_t *idx, const u
     if (!counts || !psum || !loss || (T > 0 && (!logits || !idx))) return Q36MOE_EINVAL;
     const size_t need = q36moe_balance_loss_workspace(T, n_expert);
     if (need && (!ws || ws_bytes < need)) return Q36MOE_EINVAL;
-    BalanceArgs A{logits, idx, mask, ld, T, n_expert, k, 0, coef, counts, psum, loss, static_cast<float *>(ws)};
+    BalanceArgs A{logits, idx, mask, ld, T, n_expert, k, 0, coef, counts, psum, loss, static_cast<float2 *>(ws)};
     const int nb = T ? balance_groups(T) : 1;
     A.chunk = (int)(((int64_t)T + nb - 1) / nb);
     hipStream_t s = static_cast<hipStream_t>(stream);
-    if (n_expert <= 64) hipLaunchKernelGGL(k_balance<4>, dim3(nb), dim3(64 * kBalW), 0, s, A);
-    else hipLaunchKernelGGL(k_balance<16>, dim3(nb), dim3(64 * kBalW), 0, s, A);
+    if (n_expert <= 64) hipLaunchKernelGGL(k_balance<1>, dim3(nb), dim3(64 * kBalW), 0, s, A);
+    else hipLaunchKernelGGL(k_balance<4>, dim3(nb), dim3(64 * kBalW), 0, s, A);
     if (nb > 1) hipLaunchKernelGGL(k_balance_join, dim3(1), dim3(1024), 0, s, A, nb);
     return hip_status(hipGetLastError());
 }
@@ -889,8 +1086,14 @@ int q36moe_router_topk_backward(const float *logits, int ld, const int32_t *idx,
     const int64_t nb = ((int64_t)T + 15) / 16;
     const dim3 g((unsigned)(nb < 4096 ? nb : 4096));
     hipStream_t s = static_cast<hipStream_t>(stream);
-    if (n_expert <= 64) hipLaunchKernelGGL(k_logit_grad<4>, g, dim3(256), 0, s, A);
-    else hipLaunchKernelGGL(k_logit_grad<16>, g, dim3(256), 0, s, A);
+    const bool full = counts || !renorm;
+    if (n_expert <= 64) {
+        if (full) hipLaunchKernelGGL((k_logit_grad<1, true>), g, dim3(256), 0, s, A);
+        else hipLaunchKernelGGL((k_logit_grad<1, false>), g, dim3(256), 0, s, A);
+    } else {
+        if (full) hipLaunchKernelGGL((k_logit_grad<4, true>), g, dim3(256), 0, s, A);
+        else hipLaunchKernelGGL((k_logit_grad<4, false>), g, dim3(256), 0, s, A);
+    }
     return hip_status(hipGetLastError());
 }
 
@@ -904,7 +1107,7 @@ int q36moe_router_logits_backward(const float *w, int n_rows, int n_expert, cons
                                   const float *dlogits, int ld, const float *dshg, int ld_shg, float *dw, void *dx, void *ws,
                                   size_t ws_bytes, void *stream) {
     if (T < 0 || T > kMaxRouterT || d_model != kRgD || n_expert < 1 || n_rows < n_expert || n_rows > n_expert + 1 ||
-        n_rows > kMaxRouterRows || ld < n_expert || (x_fmt != Q36MOE_FMT_F32 && x_fmt != Q36MOE_FMT_BF16) || (!dw && !dx) ||
+        n_rows > kMaxRouterRows || ld < n_expert || ld > kMaxRouterLd || (x_fmt != Q36MOE_FMT_F32 && x_fmt != Q36MOE_FMT_BF16) || (!dw && !dx) ||
         ld_shg < 0)
         return Q36MOE_EINVAL;
     hipStream_t s = static_cast<hipStream_t>(stream);

@@ -119,40 +119,63 @@ __device__ __forceinline__ float sum_rows4(float a) {
 }
 __device__ __forceinline__ float sum64(float v) { return sum_rows4(sum16(v)); }
 
-// out[c] = sum over p < P of part[p * L + c], in the order of 16 interleaved
-// groups; columns from `split` on go to out2.  64 columns per workgroup: each
-// thread adds a sixteenth of the rows of 4 of them.
-constexpr int kSumCols = 64;
+// out[c] = sum over p < P of part[p * L + c]; columns from `split` on go to
+// out2.  Many rows of few columns: a thread adds every 64th row of 4 columns, then
+// the 64 sums of a column are added, in runs of 4 and those by a tree (512 rows of
+// 3062 columns 4 us; 16 groups 12).  Few rows of many columns: 4 columns per
+// thread, one row after the other (16 rows of 526336: 5 us, 6.5 TB/s; in groups
+// as above 10).
+__global__ __launch_bounds__(256) void k_sum_rows(const float *__restrict__ part, int P, size_t L, float *__restrict__ out) {
+    const size_t c = ((size_t)blockIdx.x * 256 + threadIdx.x) * 4;
+    if (c + 4 <= L) {
+        f32x4 acc = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 16
+        for (int p = 0; p < P; p++) acc += *reinterpret_cast<const f32x4_u *>(part + (size_t)p * L + c);
+        *reinterpret_cast<f32x4_u *>(out + c) = acc;
+    } else {
+        for (size_t o = c; o < L; o++) {
+            float s = 0.0f;
+            for (int p = 0; p < P; p++) s += part[(size_t)p * L + o];
+            out[o] = s;
+        }
+    }
+}
+
 __global__ __launch_bounds__(256) void k_sum_partials(const float *__restrict__ part, int P, size_t L, size_t split,
                                                       float *__restrict__ out, float *__restrict__ out2) {
-    __shared__ __align__(16) float red[16][kSumCols];
-    const int c4 = (threadIdx.x & 15) * 4, g = threadIdx.x >> 4;
-    const size_t c = (size_t)blockIdx.x * kSumCols + c4;
+    constexpr int G = 64, C4 = 256 / G, C = 4 * C4;   // groups; columns per workgroup
+    __shared__ __align__(16) float red[G][C];
+    const int c4 = threadIdx.x % C4 * 4, g = threadIdx.x / C4;
+    const size_t c = (size_t)blockIdx.x * C + c4;
     f32x4 acc = {0.f, 0.f, 0.f, 0.f};
     if (c + 4 <= L) {
-#pragma unroll 4
-        for (int p = g; p < P; p += 16) acc += *reinterpret_cast<const f32x4_u *>(part + (size_t)p * L + c);
+#pragma unroll 8
+        for (int p = g; p < P; p += G) acc += *reinterpret_cast<const f32x4_u *>(part + (size_t)p * L + c);
     } else {
-        for (int p = g; p < P; p += 16)
+        for (int p = g; p < P; p += G)
 #pragma unroll
             for (int i = 0; i < 4; i++)
                 if (c + i < L) acc[i] += part[(size_t)p * L + c + i];
     }
     *reinterpret_cast<f32x4 *>(&red[g][c4]) = acc;
     __syncthreads();
-    if (threadIdx.x < kSumCols) {
-        const size_t o = (size_t)blockIdx.x * kSumCols + threadIdx.x;
-        float s = red[0][threadIdx.x];
+    const int col = threadIdx.x >> 4, l = threadIdx.x & 15;   // 16 lanes per column
+    float s = red[4 * l][col];
 #pragma unroll
-        for (int i = 1; i < 16; i++) s += red[i][threadIdx.x];
+    for (int i = 1; i < 4; i++) s += red[4 * l + i][col];
+    s = sum16(s);
+    const size_t o = (size_t)blockIdx.x * C + col;
+    if (l == 0) {
         if (o < split) out[o] = s;
         else if (o < L) out2[o - split] = s;
     }
 }
 
 inline void sum_partials(const float *part, int P, size_t L, size_t split, float *out, float *out2, hipStream_t s) {
-    hipLaunchKernelGGL(k_sum_partials, dim3((unsigned)((L + kSumCols - 1) / kSumCols)), dim3(256), 0, s, part, P, L, split,
-                       out, out2);
+    if (P <= 32 && L > 65536 && split == L)
+        hipLaunchKernelGGL(k_sum_rows, dim3((unsigned)((L + 1023) / 1024)), dim3(256), 0, s, part, P, L, out);
+    else
+        hipLaunchKernelGGL(k_sum_partials, dim3((unsigned)((L + 15) / 16)), dim3(256), 0, s, part, P, L, split, out, out2);
 }
 
 }  // namespace

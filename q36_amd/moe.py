@@ -579,51 +579,47 @@ def quant_e4m3(x):
 # ---------------------------------------------------------------------------
 # training what stands in front of the experts
 # ---------------------------------------------------------------------------
+# On the host a small call is a launch (2 us), an allocation per output (1.2 to
+# 1.6 us) and the checks below, whose common case is a few attribute reads.
 _FMT = {torch.float32: FMT_F32, torch.bfloat16: FMT_BF16}
+_F32 = (torch.float32,)
 
 
-def _rows(t, name, shape, dtypes, dev):
-    """(pointer, row stride) of a 2-D GPU tensor of `shape` on device `dev`
-    whose rows are contiguous and do not overlap."""
-    if not isinstance(t, torch.Tensor) or t.device != dev:
-        raise Q36MoEError(f"{name} must be a tensor on {dev}")
-    if t.dtype not in dtypes:
-        raise Q36MoEError(f"{name} must be {' or '.join(map(str, dtypes))}, got {t.dtype}")
-    if t.dim() != 2 or t.shape != shape:
-        raise Q36MoEError(f"{name} must be {list(shape)}, got {list(t.shape)}")
-    T, n = shape
-    if n > 1 and t.stride(1) != 1:
-        raise Q36MoEError(f"{name} rows must be contiguous")
-    if T < 2:
-        return t.data_ptr(), n
-    if t.stride(0) < n:
-        raise Q36MoEError(f"{name} rows must not overlap")
-    return t.data_ptr(), t.stride(0)
-
-
-def _vec(t, name, n, dtypes, dev):
-    """Pointer of a contiguous 1-D GPU tensor of n elements, or None."""
-    if t is None:
-        return None
-    if not isinstance(t, torch.Tensor) or t.device != dev or t.dtype not in dtypes or t.shape != (n,) or \
-            not t.is_contiguous():
-        raise Q36MoEError(f"{name} must be a contiguous {dtypes[0]} tensor of {n} elements on {dev}")
-    return t.data_ptr()
-
-
-def _current(t, name, dims=2):
-    """The device of `t`, which must be the current one: kernels are launched there."""
+def _gpu_of(t, name, dims=2):
+    """The GPU that `t` is on, which must be the current one: kernels are
+    launched there."""
     if not isinstance(t, torch.Tensor) or not t.is_cuda:
         raise Q36MoEError(f"{name} must be a GPU tensor")
     if t.dim() != dims:
         raise Q36MoEError(f"{name} must have {dims} dimensions")
-    if t.device.index != torch.cuda.current_device():
-        raise Q36MoEError(f"{name} is on {t.device}, the current device is cuda:{torch.cuda.current_device()}")
-    return t.device
+    gpu = t.get_device()
+    if gpu != torch._C._cuda_getDevice():
+        raise Q36MoEError(f"{name} is on cuda:{gpu}, the current device is cuda:{torch._C._cuda_getDevice()}")
+    return gpu
 
 
-def _workspace(n, dev):
-    return torch.empty(n, dtype=torch.uint8, device=dev) if n else None
+def _rows(t, name, T, n, dtypes, gpu):
+    """(pointer, row stride) of a [T, n] tensor on that GPU whose rows are
+    contiguous and do not overlap."""
+    if isinstance(t, torch.Tensor) and t.get_device() == gpu and t.dtype in dtypes and t.shape == (T, n):
+        if t.is_contiguous():
+            return t.data_ptr(), n
+        if n < 2 or t.stride(1) == 1:
+            if T < 2:
+                return t.data_ptr(), n
+            if t.stride(0) >= n:
+                return t.data_ptr(), t.stride(0)
+    raise Q36MoEError(f"{name} must be a {' or '.join(map(str, dtypes))} tensor [{T}, {n}] on cuda:{gpu} whose rows are "
+                      "contiguous and do not overlap")
+
+
+def _packed(t, name, shape, dtypes, gpu):
+    """Pointer of a contiguous tensor of that shape on that GPU; None for None."""
+    if t is None:
+        return None
+    if isinstance(t, torch.Tensor) and t.get_device() == gpu and t.dtype in dtypes and t.shape == shape and t.is_contiguous():
+        return t.data_ptr()
+    raise Q36MoEError(f"{name} must be a contiguous {' or '.join(map(str, dtypes))} tensor {list(shape)} on cuda:{gpu}")
 
 
 def _ptr(t):
@@ -634,19 +630,27 @@ def layernorm(x, w=None, b=None, a=None, eps=1e-6, rms=False, out_dtype=None):
     """Residual add + layer norm (rms: RMS norm) of rows: x, a [T, D] f32|bf16
     (rows contiguous, any row stride), w, b [D] f32 or None -> (y, h): y [T, D]
     in out_dtype (x's if None), h = x + a in x's dtype (None without a)."""
-    dev = _current(x, "x")
+    gpu = _gpu_of(x, "x")
     T, D = x.shape
-    xp, ldx = _rows(x, "x", (T, D), tuple(_FMT), dev)
-    ap, lda = (None, D) if a is None else _rows(a, "a", (T, D), (x.dtype,), dev)
-    out_dtype = out_dtype or x.dtype
-    if out_dtype not in _FMT:
+    dt = x.dtype
+    xp, ldx = _rows(x, "x", T, D, _FMT, gpu)
+    yf = _FMT.get(out_dtype or dt)
+    if yf is None:
         raise Q36MoEError("out_dtype must be float32 or bfloat16")
-    wp, bp = _vec(w, "w", D, (torch.float32,), dev), _vec(b, "b", D, (torch.float32,), dev)
-    y = torch.empty((T, D), dtype=out_dtype, device=dev)
-    h = None if a is None else torch.empty((T, D), dtype=x.dtype, device=dev)
-    check(lib().q36moe_layernorm(xp, ldx, ap, lda, _FMT[x.dtype], wp, bp, T, D, float(eps),
-                                 NORM_RMS if rms else NORM_LAYER, _ptr(h), D, y.data_ptr(), D, _FMT[out_dtype],
-                                 _stream()), "q36moe_layernorm")
+    wp = None if w is None else _packed(w, "w", (D,), _F32, gpu)
+    bp = None if b is None else _packed(b, "b", (D,), _F32, gpu)
+    y = x.new_empty((T, D), dtype=out_dtype)
+    if a is None:
+        h = hp = ap = None
+        lda = D
+    else:
+        ap, lda = _rows(a, "a", T, D, (dt,), gpu)
+        h = x.new_empty((T, D))
+        hp = h.data_ptr()
+    rc = lib().q36moe_layernorm(xp, ldx, ap, lda, _FMT[dt], wp, bp, T, D, eps, NORM_RMS if rms else NORM_LAYER, hp, D,
+                                y.data_ptr(), D, yf, _stream())
+    if rc:
+        check(rc, "q36moe_layernorm")
     return y, h
 
 
@@ -656,34 +660,46 @@ def layernorm_backward(dy, h, w=None, dres=None, eps=1e-6, rms=False, want_dx=Tr
     (the residual stream's gradient, added to dx) or None -> (dx, dw, db): dx
     [T, D] in h's dtype, dw and db [D] f32; None for what is not wanted (db is,
     by default, for a layer norm)."""
-    dev = _current(h, "h")
+    gpu = _gpu_of(h, "h")
     T, D = h.shape
-    hp, ldh = _rows(h, "h", (T, D), tuple(_FMT), dev)
-    gp, ldg = _rows(dy, "dy", (T, D), tuple(_FMT), dev)
-    rp, ldr = (None, D) if dres is None else _rows(dres, "dres", (T, D), (h.dtype,), dev)
-    wp = _vec(w, "w", D, (torch.float32,), dev)
-    dx = torch.empty((T, D), dtype=h.dtype, device=dev) if want_dx else None
-    dw = torch.empty((D,), dtype=torch.float32, device=dev) if want_dw else None
-    db = torch.empty((D,), dtype=torch.float32, device=dev) if (not rms if want_db is None else want_db) else None
+    dt = h.dtype
+    hp, ldh = _rows(h, "h", T, D, _FMT, gpu)
+    gp, ldg = _rows(dy, "dy", T, D, _FMT, gpu)
+    rp, ldr = (None, D) if dres is None else _rows(dres, "dres", T, D, (dt,), gpu)
+    wp = None if w is None else _packed(w, "w", (D,), _F32, gpu)
+    dx = h.new_empty((T, D)) if want_dx else None
+    dw = h.new_empty((D,), dtype=torch.float32) if want_dw else None
+    db = h.new_empty((D,), dtype=torch.float32) if (not rms if want_db is None else want_db) else None
     L = lib()
-    n = L.q36moe_layernorm_backward_workspace(T, D) if want_dw or db is not None else 0
-    ws = _workspace(n, dev)
-    check(L.q36moe_layernorm_backward(gp, ldg, _FMT[dy.dtype], hp, ldh, rp, ldr, _FMT[h.dtype], wp, T, D, float(eps),
-                                      NORM_RMS if rms else NORM_LAYER, _ptr(dx), D, _ptr(dw), _ptr(db), _ptr(ws), n,
-                                      _stream()), "q36moe_layernorm_backward")
+    ws = wsp = None
+    n = 0
+    if dw is not None or db is not None:
+        n = L.q36moe_layernorm_backward_workspace(T, D)
+        if n:
+            ws = h.new_empty((n,), dtype=torch.uint8)
+            wsp = ws.data_ptr()
+    rc = L.q36moe_layernorm_backward(gp, ldg, _FMT[dy.dtype], hp, ldh, rp, ldr, _FMT[dt], wp, T, D, eps,
+                                     NORM_RMS if rms else NORM_LAYER, _ptr(dx), D, _ptr(dw), _ptr(db), wsp, n, _stream())
+    if rc:
+        check(rc, "q36moe_layernorm_backward")
     return dx, dw, db
 
 
-def _mask(mask, T, dev):
-    """Pointer of the tokens' mask (bool or uint8, 0 for padding), or None."""
-    return _vec(mask, "mask", T, (torch.uint8, torch.bool), dev)
+_MASK = (torch.bool, torch.uint8)
+_I32 = (torch.int32,)
 
 
-def _picks(idx, T, dev):
-    p, _ = _rows(idx, "idx", (T, idx.shape[1] if isinstance(idx, torch.Tensor) and idx.dim() == 2 else -1), (torch.int32,), dev)
-    if not idx.is_contiguous():
-        raise Q36MoEError("idx must be contiguous")
-    return p
+def _router_args(logits, idx, mask, n_expert):
+    """What the logits' operators share: GPU, T, experts, picks, and the
+    pointers (and row stride) of logits, idx and mask."""
+    gpu = _gpu_of(logits, "logits")
+    T, E = logits.shape
+    lp, ld = _rows(logits, "logits", T, E, _F32, gpu)
+    if not isinstance(idx, torch.Tensor) or idx.dim() != 2:
+        raise Q36MoEError("idx must be a tensor [T, k]")
+    k = idx.shape[1]
+    return (gpu, T, n_expert or E, k, lp, ld, _packed(idx, "idx", (T, k), _I32, gpu),
+            None if mask is None else _packed(mask, "mask", (T,), _MASK, gpu))
 
 
 def balance_loss(logits, idx, coef=1.0, mask=None, n_expert=None):
@@ -692,19 +708,17 @@ def balance_loss(logits, idx, coef=1.0, mask=None, n_expert=None):
     (0 for padding) or None -> (loss [] f32, counts int32 [n_expert + 1], the
     last one the number of live tokens, psum f32 [n_expert], the sums of the
     tokens' softmax)."""
-    dev = _current(logits, "logits")
-    T = logits.shape[0]
-    E = n_expert or logits.shape[1]
-    lp, ld = _rows(logits, "logits", tuple(logits.shape), (torch.float32,), dev)
-    ip, mp = _picks(idx, T, dev), _mask(mask, T, dev)
-    loss = torch.empty((), dtype=torch.float32, device=dev)
-    counts = torch.empty((E + 1,), dtype=torch.int32, device=dev)
-    psum = torch.empty((E,), dtype=torch.float32, device=dev)
+    _, T, E, k, lp, ld, ip, mp = _router_args(logits, idx, mask, n_expert)
+    loss = logits.new_empty(())
+    counts = logits.new_empty((E + 1,), dtype=torch.int32)
+    psum = logits.new_empty((E,))
     L = lib()
     n = L.q36moe_balance_loss_workspace(T, E)
-    ws = _workspace(n, dev)
-    check(L.q36moe_balance_loss(lp, ld, ip, mp, T, E, idx.shape[1], float(coef), counts.data_ptr(), psum.data_ptr(),
-                                loss.data_ptr(), _ptr(ws), n, _stream()), "q36moe_balance_loss")
+    ws = logits.new_empty((n,), dtype=torch.uint8) if n else None
+    rc = L.q36moe_balance_loss(lp, ld, ip, mp, T, E, k, coef, counts.data_ptr(), psum.data_ptr(), loss.data_ptr(), _ptr(ws),
+                               n, _stream())
+    if rc:
+        check(rc, "q36moe_balance_loss")
     return loss, counts, psum
 
 
@@ -714,24 +728,15 @@ def router_topk_backward(logits, idx, dwt=None, scale=1.0, renorm=True, counts=N
     the gradient of router_topk's weights (scale and renorm as there), and, with
     the counts of balance_loss, from its loss (coef as there, dloss [] f32 its
     gradient, 1 if None).  Rows with mask 0 are zero."""
-    dev = _current(logits, "logits")
-    T = logits.shape[0]
-    E = n_expert or logits.shape[1]
-    lp, ld = _rows(logits, "logits", tuple(logits.shape), (torch.float32,), dev)
-    ip, mp = _picks(idx, T, dev), _mask(mask, T, dev)
-    k = idx.shape[1]
-    wp = None
-    if dwt is not None:
-        wp, _ = _rows(dwt, "dwt", (T, k), (torch.float32,), dev)
-        if not dwt.is_contiguous():
-            raise Q36MoEError("dwt must be contiguous")
-    cp = _vec(counts, "counts", E + 1, (torch.int32,), dev)
-    if dloss is not None and (not isinstance(dloss, torch.Tensor) or dloss.device != dev or dloss.dtype != torch.float32 or
-                              dloss.numel() != 1):
-        raise Q36MoEError(f"dloss must be one float32 value on {dev}")
-    out = torch.empty((T, E), dtype=torch.float32, device=dev)
-    check(lib().q36moe_router_topk_backward(lp, ld, ip, wp, cp, mp, _ptr(dloss), T, E, k, float(scale), 1 if renorm else 0,
-                                            float(coef), out.data_ptr(), E, _stream()), "q36moe_router_topk_backward")
+    gpu, T, E, k, lp, ld, ip, mp = _router_args(logits, idx, mask, n_expert)
+    wp = None if dwt is None else _packed(dwt, "dwt", (T, k), _F32, gpu)
+    cp = None if counts is None else _packed(counts, "counts", (E + 1,), _I32, gpu)
+    sp = None if dloss is None else _packed(dloss, "dloss", (), _F32, gpu)
+    out = logits.new_empty((T, E))
+    rc = lib().q36moe_router_topk_backward(lp, ld, ip, wp, cp, mp, sp, T, E, k, scale, 1 if renorm else 0, coef,
+                                           out.data_ptr(), E, _stream())
+    if rc:
+        check(rc, "q36moe_router_topk_backward")
     return out
 
 
@@ -740,26 +745,28 @@ def router_logits_backward(w, x, n_expert, dlogits, dshg=None, want_dw=True, wan
     dlogits [T, n_expert] f32 (row stride free) and, with n_rows == n_expert + 1,
     dshg [T] f32 (any stride) -> (dw f32 [n_rows, 2048], dx [T, 2048] in x's
     dtype; None for what is not wanted)."""
-    dev = _current(x, "x")
+    gpu = _gpu_of(x, "x")
     T, D = x.shape
+    if not isinstance(w, torch.Tensor) or w.dim() != 2:
+        raise Q36MoEError("w must be a tensor [n_rows, 2048]")
     n_rows = w.shape[0]
-    wp, _ = _rows(w, "w", (n_rows, D), (torch.float32,), dev)
-    xp, _ = _rows(x, "x", (T, D), tuple(_FMT), dev)
-    if not (w.is_contiguous() and x.is_contiguous()):
-        raise Q36MoEError("w and x must be contiguous")
-    gp, ld = _rows(dlogits, "dlogits", (T, n_expert), (torch.float32,), dev)
+    wp = _packed(w, "w", (n_rows, D), _F32, gpu)
+    xp = _packed(x, "x", (T, D), _FMT, gpu)
+    gp, ld = _rows(dlogits, "dlogits", T, n_expert, _F32, gpu)
     if (dshg is None) != (n_rows == n_expert):
         raise Q36MoEError("dshg goes with the shared gate's row")
-    if dshg is not None and dshg.device != dev:
-        raise Q36MoEError(f"dshg must be on {dev}")
     sp, lds = _shg(dshg, T)
-    dw = torch.empty((n_rows, D), dtype=torch.float32, device=dev) if want_dw else None
-    dx = torch.empty((T, D), dtype=x.dtype, device=dev) if want_dx else None
+    if dshg is not None and dshg.get_device() != gpu:
+        raise Q36MoEError(f"dshg must be on cuda:{gpu}")
+    dw = w.new_empty((n_rows, D)) if want_dw else None
+    dx = x.new_empty((T, D)) if want_dx else None
     L = lib()
     n = L.q36moe_router_logits_backward_workspace(T, n_rows) if want_dw else 0
-    ws = _workspace(n, dev)
-    check(L.q36moe_router_logits_backward(wp, n_rows, n_expert, xp, _FMT[x.dtype], T, D, gp, ld, sp, lds, _ptr(dw),
-                                          _ptr(dx), _ptr(ws), n, _stream()), "q36moe_router_logits_backward")
+    ws = x.new_empty((n,), dtype=torch.uint8) if n else None
+    rc = L.q36moe_router_logits_backward(wp, n_rows, n_expert, xp, _FMT[x.dtype], T, D, gp, ld, sp, lds, _ptr(dw), _ptr(dx),
+                                         _ptr(ws), n, _stream())
+    if rc:
+        check(rc, "q36moe_router_logits_backward")
     return dw, dx
 
 

@@ -490,7 +490,8 @@ def test_router_topk_backward_strided_rows_keep_their_surroundings(dev):
 @pytest.mark.parametrize("T,E,shared", [(1, 1, False), (1, 256, True), (2, 7, True), (17, 256, True), (31, 33, False),
                                         (33, 8, True), (64, 255, False), (100, 32, True), (203, 256, True), (257, 257, True),
                                         (300, 300, False), (513, 256, False), (700, 60, True), (1025, 256, True),
-                                        (1100, 600, True), (2500, 128, True), (4097, 256, True)])
+                                        (1100, 600, True), (2500, 128, True), (4097, 256, True), (640, 256, True), (641, 131, False),
+                                        (1025, 65, True), (1401, 20, True), (3001, 7, False)])
 @pytest.mark.parametrize("xt", [F32, BF16])
 def test_router_logits_backward(dev, T, E, shared, xt):
     g = _g(T * 1000 + E)
