@@ -25,17 +25,6 @@ __device__ __forceinline__ void wave_sync() {
     __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
 }
 
-// exp(x) for x <= 0 as 2^hi * (1 + lo ln 2), hi + lo = x log2(e) to 48 bits:
-// about 1 ulp however large -x is.
-__device__ __forceinline__ float exp_neg(float x) {
-    constexpr float kL = 1.44269502162933349609f, kLl = 1.92596299112661746887e-8f;   // log2(e) in two floats
-    const float hi = x * kL;
-    const float lo = fmaf(x, kLl, fmaf(x, kL, -hi));
-    const float e = __builtin_amdgcn_exp2f(hi);
-    // x = -inf gives lo = NaN where e is 0 already
-    return e == 0.0f ? 0.0f : fmaf(e, lo * 0.693147180559945309417f, e);
-}
-
 // A token's E values in 16 lanes: lane l holds columns 64 i + 4 l..+3 in v[i],
 // so that rows move as 16-byte vectors where E is a multiple of 4 (whatever
 // their alignment) and as single values elsewhere.  Columns past E read as
@@ -76,10 +65,12 @@ __device__ __forceinline__ void store16(float *__restrict__ row, int E, int l, c
     }
 }
 
-// Softmax of the values that 16 lanes hold; m and s are left to the caller.  A
-// row of -inf has no probabilities: all 0.
+// Softmax of the values that 16 lanes hold: v becomes exp(v - max), and one over
+// their sum is returned; a row of -inf has no probabilities, all 0.  Two roundings
+// of the exponent, 2^-23 |v - max| of the value.
 template <int NV, int NC>
-__device__ __forceinline__ void softmax16(float (&v)[NV][NC]) {
+__device__ __forceinline__ float softmax16(float (&v)[NV][NC]) {
+    constexpr float kLog2e = 1.44269504088896341f;
     float m = v[0][0];
 #pragma unroll
     for (int i = 0; i < NV; i++)
@@ -92,15 +83,11 @@ __device__ __forceinline__ void softmax16(float (&v)[NV][NC]) {
     for (int i = 0; i < NV; i++)
 #pragma unroll
         for (int c = 0; c < NC; c++) {
-            v[i][c] = exp_neg(v[i][c] - m);
+            v[i][c] = __builtin_amdgcn_exp2f((v[i][c] - m) * kLog2e);
             s += v[i][c];
         }
     s = sum16(s);
-    const float inv = s == 0.0f ? 0.0f : 1.0f / s;   // a NaN stays one
-#pragma unroll
-    for (int i = 0; i < NV; i++)
-#pragma unroll
-        for (int c = 0; c < NC; c++) v[i][c] *= inv;
+    return s == 0.0f ? 0.0f : 1.0f / s;   // a NaN stays one
 }
 
 template <int NV>
@@ -124,37 +111,40 @@ struct BalanceArgs {
     float coef;
     int32_t *counts;           // [E + 1]
     float *psum, *loss;        // [E], [1]
-    float2 *part;              // [workgroups][E + 1]: sum of probabilities, count
+    // of more than one workgroup: [workgroups][E + 1] sum of probabilities and
+    // count, then a partial loss per joining workgroup, live tokens, arrivals
+    float2 *part;
 };
 
-// loss from counts and sums by the first wave, in 64 bits: counts times sums of
-// probabilities over many tokens.
-__device__ __forceinline__ void balance_of(const BalanceArgs &A, const int32_t *cnt, const float *ps) {
-    if (threadIdx.x < 64) {
-        double s = 0.0;
-#pragma unroll
-        for (int i = 0; i < kMaxE / 64; i++) {
-            const int e = threadIdx.x + 64 * i;
-            if (e < A.E) s += (double)cnt[e] * (double)ps[e];
-        }
-#pragma unroll
-        for (int o = 32; o > 0; o >>= 1) s += __shfl_xor(s, o, 64);
-        const double n = (double)cnt[A.E];
-        if (threadIdx.x == 0) *A.loss = n > 0.0 ? (float)((double)A.coef * A.E * s / ((double)A.k * n * n)) : 0.0f;
-    }
+constexpr int kBalW = 16;                        // waves per workgroup
+constexpr int kBalGroups = 256;                  // most workgroups
+constexpr int kJoinE = 16;                       // counters per joining workgroup
+constexpr int kJoins = (kMaxE + 1 + kJoinE - 1) / kJoinE;
+struct BalanceJoin {
+    double loss[kJoins];
+    int32_t live, arrived;
+};
+__host__ __device__ inline size_t balance_part_bytes(int nb, int E) { return ((size_t)nb * (E + 1) * sizeof(float2) + 15) / 16 * 16; }
+
+// coef * E / (k n^2) times the sum of counts times sums of probabilities, which
+// is formed in 64 bits.
+__device__ __forceinline__ float balance_of(const BalanceArgs &A, double s, int32_t live) {
+    const double n = (double)live;
+    return live > 0 ? (float)((double)A.coef * A.E * s / ((double)A.k * n * n)) : 0.0f;
 }
 
-constexpr int kBalW = 16;   // waves per workgroup
-
 // 16 lanes per token, 64 tokens of the workgroup's run at a time, the next
-// token's loads ahead of the sums of this one.  A token of padding is a row of
-// -inf without picks.
+// token's loads ahead of the sums of this one.  What bounds a workgroup is the
+// vector unit: 64 tokens of 256 experts take a CU 1.4 us, so the tokens are spread
+// over all of them.
 template <int NV>
 __global__ __launch_bounds__(64 * kBalW) void k_balance(BalanceArgs A) {
     __shared__ __align__(16) float ps[kBalW][64 * NV];
     __shared__ int32_t cnt[kMaxE + 1];
     const int tid = threadIdx.x, l = tid & 15, wave = tid >> 6;
     const int64_t t0 = (int64_t)blockIdx.x * A.chunk, t1 = min(t0 + A.chunk, (int64_t)A.T);
+    if (gridDim.x > 1 && blockIdx.x == 0 && tid == 0)   // for the joining kernel, which runs after this one
+        reinterpret_cast<BalanceJoin *>(reinterpret_cast<uint8_t *>(A.part) + balance_part_bytes(gridDim.x, A.E))->arrived = 0;
     for (int e = tid; e <= A.E; e += 64 * kBalW) cnt[e] = 0;
     __syncthreads();
     float acc[NV][4] = {}, v[NV][4];
@@ -176,17 +166,19 @@ __global__ __launch_bounds__(64 * kBalW) void k_balance(BalanceArgs A) {
 #pragma unroll
         for (int i = 0; i < NV; i++)
 #pragma unroll
-            for (int c = 0; c < 4; c++) p[i][c] = live ? v[i][c] : -INFINITY;
-        if (live) {
+            for (int c = 0; c < 4; c++) p[i][c] = v[i][c];
+        const bool counted = live;
+        if (counted) {
             if ((unsigned)pick < (unsigned)A.E) atomicAdd(&cnt[pick], 1);
             n += l == 0;
         }
         load(t + 4 * kBalW);
-        softmax16(p);
+        const float inv = softmax16(p);
+        if (counted)   // padding may hold anything
 #pragma unroll
-        for (int i = 0; i < NV; i++)
+            for (int i = 0; i < NV; i++)
 #pragma unroll
-            for (int c = 0; c < 4; c++) acc[i][c] += p[i][c];
+                for (int c = 0; c < 4; c++) acc[i][c] = fmaf(p[i][c], inv, acc[i][c]);
     }
     if (n) atomicAdd(&cnt[A.E], n);
 #pragma unroll
@@ -214,49 +206,71 @@ __global__ __launch_bounds__(64 * kBalW) void k_balance(BalanceArgs A) {
     }
     if (e <= A.E) A.counts[e] = cnt[e];
     __syncthreads();
-    balance_of(A, cnt, ps[0]);
+    if (wave == 0) {
+        double d = 0.0;
+#pragma unroll
+        for (int i = 0; i < kMaxE / 64; i++)
+            if (tid + 64 * i < A.E) d += (double)cnt[tid + 64 * i] * (double)ps[0][tid + 64 * i];
+#pragma unroll
+        for (int o = 32; o > 0; o >>= 1) d += __shfl_xor(d, o, 64);
+        if (tid == 0) *A.loss = balance_of(A, d, cnt[A.E]);
+    }
 }
 
-// The workgroups' parts to counts, sums and loss: thread (group of parts, expert).
-constexpr int kBalGroups = 128;   // most parts
-__global__ __launch_bounds__(1024) void k_balance_join(BalanceArgs A, int nb) {
-    __shared__ float ps[4][kMaxE + 1];
-    __shared__ int32_t cs[4][kMaxE + 1];
-    const int n = A.E + 1;
-    auto add = [&](int e, int g) {
-        float s = 0.0f;
-        int32_t c = 0;
+// The workgroups' parts to counts, sums and loss, 16 counters per workgroup (one
+// CU alone brings 50 GB/s in: 128 parts took it 6.8 us).  The workgroup that
+// arrives last adds the partial losses, in the order of the experts.
+__global__ __launch_bounds__(256) void k_balance_join(BalanceArgs A, int nb) {
+    __shared__ float ps[16][kJoinE];
+    __shared__ int32_t cs[16][kJoinE];
+    __shared__ int last;
+    BalanceJoin *J = reinterpret_cast<BalanceJoin *>(reinterpret_cast<uint8_t *>(A.part) + balance_part_bytes(nb, A.E));
+    const int c = threadIdx.x & 15, g = threadIdx.x >> 4, e = blockIdx.x * kJoinE + c, n = A.E + 1;
+    float s = 0.0f;
+    int32_t k = 0;
+    if (e < n)
 #pragma unroll 16
-        for (int b = g; b < nb; b += 4) {
+        for (int b = g; b < nb; b += 16) {
             const float2 v = A.part[(size_t)b * n + e];
             s += v.x;
-            c += __float_as_int(v.y);
+            k += __float_as_int(v.y);
         }
-        ps[g][e] = s;
-        cs[g][e] = c;
-    };
-    const int e = threadIdx.x & 255, g = threadIdx.x >> 8;
-    if (e < n) add(e, g);
-    if (n == 257 && e == 0) add(256, g);
+    ps[g][c] = s;
+    cs[g][c] = k;
     __syncthreads();
-    for (int i = threadIdx.x; i < n; i += 1024) {
-        const int32_t c = cs[0][i] + cs[1][i] + cs[2][i] + cs[3][i];
-        cs[0][i] = c;
-        A.counts[i] = c;
-        if (i < A.E) {
-            const float s = (ps[0][i] + ps[1][i]) + (ps[2][i] + ps[3][i]);
-            ps[0][i] = s;
-            A.psum[i] = s;
+    if (threadIdx.x < kJoinE) {
+        s = 0.0f;
+        k = 0;
+#pragma unroll
+        for (int i = 0; i < 16; i++) {
+            s += ps[i][c];
+            k += cs[i][c];
         }
+        if (e < n) A.counts[e] = k;
+        if (e < A.E) A.psum[e] = s;
+        double d = e < A.E ? (double)k * (double)s : 0.0;
+#pragma unroll
+        for (int o = 8; o > 0; o >>= 1) d += __shfl_xor(d, o, 16);
+        if (e == A.E) __hip_atomic_store(&J->live, k, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        if (c == 0) __hip_atomic_store(&J->loss[blockIdx.x], d, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        __threadfence();
+        if (c == 0) last = __hip_atomic_fetch_add(&J->arrived, 1, __ATOMIC_ACQ_REL, __HIP_MEMORY_SCOPE_AGENT) == (int)gridDim.x - 1;
     }
     __syncthreads();
-    balance_of(A, cs[0], ps[0]);
+    if (threadIdx.x == 0 && last) {
+        __threadfence();
+        double d = 0.0;
+        for (int b = 0; b < (int)gridDim.x; b++) d += __hip_atomic_load(&J->loss[b], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        *A.loss = balance_of(A, d, __hip_atomic_load(&J->live, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT));
+    }
 }
 
-// Workgroups: one up to 128 tokens (no second launch), then 64 tokens each up to
-// kBalGroups of them, whose parts one workgroup still joins in a few microseconds.
+// Workgroups: one up to 384 tokens, which saves the second launch and the
+// workspace, then one per 64 tokens, and from 16384 tokens on one per CU.  us on the
+// GPU, one workgroup / more: 256 tokens 9.6 / 11.1, 400 12.6 / 11.3, 600 16.8 / 11.2;
+// at 32768 tokens 64 / 128 / 256 workgroups 23.1 / 18.3 / 14.6.
 int balance_groups(int T) {
-    if (T <= 128) return 1;
+    if (T <= 384) return 1;
     const int n = (int)(((int64_t)T + 63) / 64);
     return n < kBalGroups ? n : kBalGroups;
 }
@@ -316,9 +330,9 @@ __global__ __launch_bounds__(256) void k_logit_grad(LogitGradArgs A) {
             float s = e >= 0 ? up : 0.0f;
             if (A.renorm) {
                 float q[1][1] = {{lp}};
-                softmax16(q);
-                const float mean = sum16(q[0][0] * s);   // by all 16 lanes, those without a pick too
-                s = e >= 0 ? q[0][0] * (up - mean) : 0.0f;
+                const float share = softmax16(q) * q[0][0];
+                const float mean = sum16(share * s);   // by all 16 lanes, those without a pick too
+                s = e >= 0 ? share * (up - mean) : 0.0f;
             }
             // the same expert at two slots of a token: compared with the lanes
             // 1..7 to the right in the row
@@ -353,15 +367,16 @@ __global__ __launch_bounds__(256) void k_logit_grad(LogitGradArgs A) {
                 for (int c = 0; c < 4; c++) u[i][c] = 0.0f;
         }
         if (FULL) {
-            softmax16(p);
-            const float d = balance ? dot16(p, f) : 0.0f;
-            const float du = A.dwt && !A.renorm ? dot16(p, u) : 0.0f;
+            const float inv = softmax16(p);
+            const float d = balance ? dot16(p, f) * inv : 0.0f;
+            const float du = A.dwt && !A.renorm ? dot16(p, u) * inv : 0.0f;
+            const float gi = gain * inv;
 #pragma unroll
             for (int i = 0; i < NV; i++)
 #pragma unroll
                 for (int c = 0; c < 4; c++) {
-                    if (!A.renorm) u[i][c] = p[i][c] * (u[i][c] - du);
-                    if (balance) u[i][c] = fmaf(gain * p[i][c], f[i][c] - d, u[i][c]);
+                    if (!A.renorm) u[i][c] = p[i][c] * inv * (u[i][c] - du);
+                    if (balance) u[i][c] = fmaf(gi * p[i][c], f[i][c] - d, u[i][c]);
                 }
         }
 #pragma unroll
@@ -1054,7 +1069,7 @@ extern "C" {
 size_t q36moe_balance_loss_workspace(int T, int n_expert) {
     if (T < 1 || n_expert < 1 || n_expert > kMaxE) return 0;
     const int nb = balance_groups(T);
-    return nb == 1 ? 0 : (size_t)nb * (n_expert + 1) * sizeof(float2);
+    return nb == 1 ? 0 : balance_part_bytes(nb, n_expert) + sizeof(BalanceJoin);
 }
 
 int q36moe_balance_loss(const float *logits, int ld, const int32_t *idx, const uint8_t *mask, int T, int n_expert, int k,
@@ -1070,7 +1085,7 @@ int q36moe_balance_loss(const float *logits, int ld, const int32_t *idx, const u
     hipStream_t s = static_cast<hipStream_t>(stream);
     if (n_expert <= 64) hipLaunchKernelGGL(k_balance<1>, dim3(nb), dim3(64 * kBalW), 0, s, A);
     else hipLaunchKernelGGL(k_balance<4>, dim3(nb), dim3(64 * kBalW), 0, s, A);
-    if (nb > 1) hipLaunchKernelGGL(k_balance_join, dim3(1), dim3(1024), 0, s, A, nb);
+    if (nb > 1) hipLaunchKernelGGL(k_balance_join, dim3((n_expert + kJoinE) / kJoinE), dim3(256), 0, s, A, nb);
     return hip_status(hipGetLastError());
 }
 

@@ -299,7 +299,8 @@ def _p_err(l):
 
 
 ROUTE_SHAPES = [(1, 1, 1), (1, 8, 8), (2, 3, 2), (15, 17, 1), (16, 16, 3), (17, 60, 4), (64, 64, 8), (61, 65, 5),
-                (203, 256, 8), (256, 255, 7), (257, 256, 8), (1000, 129, 6), (16500, 256, 8)]
+                (203, 256, 8), (256, 255, 7), (257, 256, 8), (384, 100, 2), (385, 256, 8), (390, 1, 1),
+                (1000, 129, 6), (16500, 256, 8)]
 
 
 @pytest.mark.parametrize("T,E,k", ROUTE_SHAPES)
