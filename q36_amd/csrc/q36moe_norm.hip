@@ -25,6 +25,7 @@ struct NormArgs {
     size_t pstride;
     int64_t ld_x, ld_a, ld_dy, ld_h, ld_y;
     int T, D, rms;
+    int streams;               // backward
     float eps, inv_d;
 };
 
@@ -41,7 +42,7 @@ __device__ __forceinline__ void row_sums(float (&s)[N], float (*red)[N * NW], in
         if ((threadIdx.x & 63) == 0)
 #pragma unroll
             for (int i = 0; i < N; i++) red[p][i * NW + wave] = s[i];
-        __syncthreads();
+        lds_barrier();
 #pragma unroll
         for (int i = 0; i < N; i++) {
             s[i] = red[p][i * NW];
@@ -152,19 +153,49 @@ __global__ __launch_bounds__(NW == 1 ? 256 : 64 * NW) void k_layernorm_backward(
     const int tid = NW == 1 ? threadIdx.x & 63 : threadIdx.x;
     const int stream = blockIdx.x * RPB + (NW == 1 ? threadIdx.x >> 6 : 0);
     int p1 = 0, p4 = 0;
-    float sw[NV][VEC], sb[NV][VEC];
+    float sw[NV][VEC], sb[NV][VEC], w[NV][VEC];
 #pragma unroll
-    for (int j = 0; j < NV; j++)
+    for (int j = 0; j < NV; j++) {
 #pragma unroll
-        for (int i = 0; i < VEC; i++) sw[j][i] = sb[j][i] = 0.0f;
-    for (int64_t t = stream; t < A.T; t += (int64_t)gridDim.x * RPB) {
-        float v[NV][VEC], g[NV][VEC], w[NV][VEC];
+        for (int i = 0; i < VEC; i++) {
+            sw[j][i] = sb[j][i] = 0.0f;
+            w[j][i] = 1.0f;
+        }
+        if (A.w) load_row<Q36MOE_FMT_F32>(A.w, Cols<VEC, TPR>(j, tid, A.D).at, w[j]);
+    }
+    // a row's loads are made before the sums of the row before it (past the last
+    // row it is read again), where registers allow
+    constexpr bool AHEAD = NV * VEC <= 16;
+    Bits<XF, VEC> bx[NV], ba[NV];
+    Bits<YF, VEC> bg[NV];
+    auto load = [&](int64_t t) {
+        t = min(t, (int64_t)A.T - 1);
 #pragma unroll
         for (int j = 0; j < NV; j++) {
             const Cols<VEC, TPR> c(j, tid, A.D);
-            load_row<XF>(A.x, t * A.ld_x + c.at, v[j]);
-            load_row<YF>(A.dy, t * A.ld_dy + c.at, g[j]);
+            bx[j].load(A.x, t * A.ld_x + c.at);
+            bg[j].load(A.dy, t * A.ld_dy + c.at);
         }
+        if (A.a)
+#pragma unroll
+            for (int j = 0; j < NV; j++) ba[j].load(A.a, t * A.ld_a + Cols<VEC, TPR>(j, tid, A.D).at);
+    };
+    if (AHEAD) load(stream);
+    const int64_t stride = (int64_t)gridDim.x * RPB;
+    for (int64_t t = stream; t < A.T; t += stride) {
+        float v[NV][VEC], g[NV][VEC];
+        Bits<XF, VEC> res[NV];
+        if (!AHEAD) load(t);
+#pragma unroll
+        for (int j = 0; j < NV; j++) {
+            res[j] = ba[j];
+#pragma unroll
+            for (int i = 0; i < VEC; i++) {
+                v[j][i] = bx[j][i];
+                g[j][i] = bg[j][i];
+            }
+        }
+        if (AHEAD) load(t + stride);
         float m0 = 0.0f;
         if (!A.rms) {
             float s[1] = {0.0f};
@@ -183,9 +214,6 @@ __global__ __launch_bounds__(NW == 1 ? 256 : 64 * NW) void k_layernorm_backward(
 #pragma unroll
         for (int j = 0; j < NV; j++) {
             const Cols<VEC, TPR> c(j, tid, A.D);
-#pragma unroll
-            for (int i = 0; i < VEC; i++) w[j][i] = 1.0f;
-            if (A.w) load_row<Q36MOE_FMT_F32>(A.w, c.at, w[j]);
 #pragma unroll
             for (int i = 0; i < VEC; i++) {
                 const float d = i >= c.skip ? v[j][i] - m0 : 0.0f;
@@ -213,16 +241,9 @@ __global__ __launch_bounds__(NW == 1 ? 256 : 64 * NW) void k_layernorm_backward(
                 sw[j][i] = fmaf(g[j][i], n, sw[j][i]);
                 sb[j][i] += g[j][i];
                 o[i] = (fmaf(g[j][i], w[j][i], -mg) - n * mgn) * r;
+                if (A.a) o[i] += res[j][i];
             }
-            if (A.y && c.skip < VEC) {
-                if (A.a) {
-                    float a[VEC];
-                    load_row<XF>(A.a, t * A.ld_a + c.at, a);
-#pragma unroll
-                    for (int i = 0; i < VEC; i++) o[i] += a[i];
-                }
-                store_row<XF>(A.y, t * A.ld_y + c.at, o, c.skip);
-            }
+            if (A.y && c.skip < VEC) store_row<XF>(A.y, t * A.ld_y + c.at, o, c.skip);
         }
     }
     if (stream >= A.T) return;   // the last workgroup's waves past the last row have no partial row
@@ -237,25 +258,29 @@ __global__ __launch_bounds__(NW == 1 ? 256 : 64 * NW) void k_layernorm_backward(
 }
 
 // Rows of up to 512 columns go to one wave, longer ones to a workgroup of 4
-// waves, past 8192 of 8.
+// waves, past 4096 of 8: 4 to 16 values of each input per thread, 32 past 8192.
 constexpr int kWaveRow = 512;
-constexpr int kMaxStreams = 512;   // streams of the backward pass, each with a row of partial sums
+// Streams of the backward pass, each with a row of partial sums that is written
+// and read again: a row of tokens each up to 256, then 4 rows and more.  256 of
+// them (one workgroup per CU) have enough in flight where a row is 16 KiB and more,
+// 512 below that: us at 16384 tokens with 256 / 512 / 1024 streams, 2048 columns
+// fp32 97 / 102 / 112, bf16 77 / 58 / 63, 4096 columns fp32 with bf16 dy
+// 174 / 183 / 190 (without the loads ahead 292 / 198 / 220).  Past 256 a multiple of
+// 4: the four waves of a workgroup are streams where NW is 1, and each has rows.
+constexpr int kMaxStreams = 512;
 
-// A row each up to 256 tokens, then 4 rows and more: a stream's partial row is
-// written and read again, as much as half a token's own traffic.  Past 256 a
-// multiple of 4: the four waves of a workgroup are streams where NW is 1, and
-// every one of them has rows.
-int streams(int T) {
+int streams(int T, size_t row_bytes) {
+    const int most = row_bytes >= 16384 ? kMaxStreams / 2 : kMaxStreams;
     if (T <= kMaxStreams / 2) return T;
     const int n = (int)(((int64_t)T + 15) / 16) * 4;
-    return n < kMaxStreams / 2 ? kMaxStreams / 2 : n < kMaxStreams ? n : kMaxStreams;
+    return n < kMaxStreams / 2 ? kMaxStreams / 2 : n < most ? n : most;
 }
 
 template <bool BWD, int XF, int YF, int VEC, int NW, int NV>
 void launch_norm(const NormArgs &A, hipStream_t s) {
     constexpr int RPB = NW == 1 ? 4 : 1;
     if constexpr (BWD)
-        hipLaunchKernelGGL((k_layernorm_backward<XF, YF, VEC, NW, NV>), dim3((streams(A.T) + RPB - 1) / RPB),
+        hipLaunchKernelGGL((k_layernorm_backward<XF, YF, VEC, NW, NV>), dim3((A.streams + RPB - 1) / RPB),
                            dim3(NW == 1 ? 256 : 64 * NW), 0, s, A);
     else
         hipLaunchKernelGGL((k_layernorm<XF, YF, VEC, NW, NV>), dim3(((A.T < (1 << 20) ? A.T : (1 << 20)) + RPB - 1) / RPB),
@@ -273,7 +298,7 @@ void norm_by_width(const NormArgs &A, hipStream_t s) {
     else if (D <= 1024 * B) launch_norm<BWD, XF, YF, VEC, 4, 1>(A, s);
     else if (D <= 2048 * B) launch_norm<BWD, XF, YF, VEC, 4, 2>(A, s);
     else if (D <= 4096 * B) launch_norm<BWD, XF, YF, VEC, 4, 4>(A, s);
-    else if (D <= 8192) launch_norm<BWD, XF, YF, VEC, 4, 8 / B>(A, s);
+    else if (D <= 8192) launch_norm<BWD, XF, YF, VEC, 8, 4 / B>(A, s);
     else launch_norm<BWD, XF, YF, VEC, 8, 8 / B>(A, s);
 }
 
@@ -317,7 +342,7 @@ int q36moe_layernorm(const void *x, int64_t ld_x, const void *a, int64_t ld_a, i
 
 size_t q36moe_layernorm_backward_workspace(int T, int d_model) {
     if (T < 2 || d_model < 1 || d_model > kMaxNormD) return 0;
-    return (size_t)streams(T) * 2 * d_model * sizeof(float);
+    return (size_t)streams(T, 0) * 2 * d_model * sizeof(float);   // the most, whatever the formats
 }
 
 int q36moe_layernorm_backward(const void *dy, int64_t ld_dy, int y_fmt, const void *h, int64_t ld_h, const void *dres,
@@ -333,19 +358,22 @@ int q36moe_layernorm_backward(const void *dy, int64_t ld_dy, int y_fmt, const vo
     hipStream_t s = static_cast<hipStream_t>(stream);
     const size_t D = (size_t)d_model;
     const size_t L = D * ((dw ? 1 : 0) + (db ? 1 : 0));
+    const int xb = x_fmt == Q36MOE_FMT_F32 ? 4 : 2, yb = y_fmt == Q36MOE_FMT_F32 ? 4 : 2;
+    const int n = streams(T, D * (2 * xb + yb));
     if (T > 0) {
         NormArgs A{};
         A.x = h; A.a = dres; A.dy = dy; A.y = dx; A.w = w;
         A.ld_x = ld_h; A.ld_a = ld_dres; A.ld_dy = ld_dy; A.ld_y = ld_dx;
         A.T = T; A.D = d_model; A.rms = kind == Q36MOE_NORM_RMS; A.eps = eps; A.inv_d = 1.0f / (float)d_model;
         A.pstride = L;
+        A.streams = n;
         float *p = static_cast<float *>(ws);
         A.pw = !dw ? nullptr : T == 1 ? dw : p;   // one stream's partial row is the sum
         A.pb = !db ? nullptr : T == 1 ? db : p + (dw ? D : 0);
         norm_by_format<true>(A, x_fmt, y_fmt, s);
     }
     // no tokens: sums of nothing
-    if (sums && T != 1) sum_partials(static_cast<const float *>(ws), T ? streams(T) : 0, L, dw ? D : 0, dw, db, s);
+    if (sums && T != 1) sum_partials(static_cast<const float *>(ws), n, L, dw ? D : 0, dw, db, s);
     return hip_status(hipGetLastError());
 }
 

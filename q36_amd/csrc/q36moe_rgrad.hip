@@ -413,8 +413,6 @@ struct ProductArgs {
 // 4 (L / 32) + i % 4 of column L % 32 in lane L.
 __device__ __forceinline__ int c_row(int i, int lane) { return 8 * (i >> 2) + 4 * (lane >> 5) + (i & 3); }
 
-// Workgroup barrier for LDS data only: prefetched global loads stay in flight.
-__device__ __forceinline__ void lds_barrier() { asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
 
 // Workgroup b of n in an order in which those of one XCD (b % 8) are neighbours.
 __device__ __forceinline__ int xcd_order(int b, int n) { return (n & 7) ? b : (b & 7) * (n >> 3) + (b >> 3); }

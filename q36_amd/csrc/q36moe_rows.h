@@ -60,6 +60,44 @@ __device__ __forceinline__ void load_row(const void *p, size_t at, float (&v)[N]
     }
 }
 
+// The same in two halves, for loads that are to be in flight while other work is
+// done: the bits, and later their values.
+template <int F, int N>
+struct Bits {
+    static constexpr int W = F == Q36MOE_FMT_F32 ? N : (N + 1) / 2;
+    uint32_t u[W];
+    __device__ __forceinline__ void load(const void *p, size_t at) {
+        if constexpr (F == Q36MOE_FMT_F32) {
+            const float *f = static_cast<const float *>(p) + at;
+            if constexpr (N == 1) {
+                u[0] = __float_as_uint(*f);
+            } else {
+#pragma unroll
+                for (int i = 0; i < N; i += 4) {
+                    const f32x4 t = *reinterpret_cast<const f32x4_u *>(f + i);
+#pragma unroll
+                    for (int j = 0; j < 4; j++) u[i + j] = __float_as_uint(t[j]);
+                }
+            }
+        } else {
+            const uint16_t *h = static_cast<const uint16_t *>(p) + at;
+            if constexpr (N == 1) {
+                u[0] = *h;
+            } else if constexpr (N == 4) {
+                const u32x2_u t = *reinterpret_cast<const u32x2_u *>(h);
+                u[0] = t[0]; u[1] = t[1];
+            } else {
+                const u32x4_u t = *reinterpret_cast<const u32x4_u *>(h);
+                u[0] = t[0]; u[1] = t[1]; u[2] = t[2]; u[3] = t[3];
+            }
+        }
+    }
+    __device__ __forceinline__ float operator[](int i) const {
+        if constexpr (F == Q36MOE_FMT_F32) return __uint_as_float(u[i]);
+        else return i & 1 ? bf16_hi(u[i / 2]) : bf16_lo(u[i / 2]);
+    }
+};
+
 template <int F>
 __device__ __forceinline__ void store_one(void *p, size_t at, float v) {
     if constexpr (F == Q36MOE_FMT_F32) static_cast<float *>(p)[at] = v;
@@ -88,6 +126,9 @@ __device__ __forceinline__ void store_row(void *p, size_t at, const float (&v)[N
                                                       bf16_pair(v[4], v[5]), bf16_pair(v[6], v[7])};
     }
 }
+
+// Workgroup barrier for LDS data only: prefetched global loads stay in flight.
+__device__ __forceinline__ void lds_barrier() { asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
 
 template <int CTRL>
 __device__ __forceinline__ float dpp(float v) {
