@@ -579,23 +579,28 @@ def quant_e4m3(x):
 # ---------------------------------------------------------------------------
 # training what stands in front of the experts
 # ---------------------------------------------------------------------------
-# On the host a small call is a launch (2 us), an allocation per output (1.2 to
-# 1.6 us) and the checks below, whose common case is a few attribute reads.
+# On the host a small call is a launch (2 us), an allocation per output (1.2 us;
+# empty_like is the cheapest form) and the checks below, whose common case is a few
+# attribute reads.
 _FMT = {torch.float32: FMT_F32, torch.bfloat16: FMT_BF16}
 _F32 = (torch.float32,)
+_raw_stream = torch._C._cuda_getCurrentRawStream
 
 
-def _gpu_of(t, name, dims=2):
-    """The GPU that `t` is on, which must be the current one: kernels are
-    launched there."""
+def _matrix(t, name, dtypes):
+    """(GPU, T, n, pointer, row stride) of a 2-D tensor on the current GPU, where
+    kernels are launched, whose rows are contiguous and do not overlap."""
     if not isinstance(t, torch.Tensor) or not t.is_cuda:
         raise Q36MoEError(f"{name} must be a GPU tensor")
-    if t.dim() != dims:
-        raise Q36MoEError(f"{name} must have {dims} dimensions")
+    if t.dim() != 2:
+        raise Q36MoEError(f"{name} must have 2 dimensions")
     gpu = t.get_device()
     if gpu != torch._C._cuda_getDevice():
         raise Q36MoEError(f"{name} is on cuda:{gpu}, the current device is cuda:{torch._C._cuda_getDevice()}")
-    return gpu
+    T, n = t.shape
+    if t.is_contiguous() and t.dtype in dtypes:
+        return gpu, T, n, t.data_ptr(), n
+    return (gpu, T, n, *_rows(t, name, T, n, dtypes, gpu))
 
 
 def _rows(t, name, T, n, dtypes, gpu):
@@ -611,6 +616,11 @@ def _rows(t, name, T, n, dtypes, gpu):
                 return t.data_ptr(), t.stride(0)
     raise Q36MoEError(f"{name} must be a {' or '.join(map(str, dtypes))} tensor [{T}, {n}] on cuda:{gpu} whose rows are "
                       "contiguous and do not overlap")
+
+
+def _like(t, dtype=None):
+    """An uninitialised contiguous tensor of t's shape."""
+    return torch.empty_like(t, dtype=dtype) if t.is_contiguous() else t.new_empty(t.shape, dtype=dtype)
 
 
 def _packed(t, name, shape, dtypes, gpu):
@@ -630,25 +640,23 @@ def layernorm(x, w=None, b=None, a=None, eps=1e-6, rms=False, out_dtype=None):
     """Residual add + layer norm (rms: RMS norm) of rows: x, a [T, D] f32|bf16
     (rows contiguous, any row stride), w, b [D] f32 or None -> (y, h): y [T, D]
     in out_dtype (x's if None), h = x + a in x's dtype (None without a)."""
-    gpu = _gpu_of(x, "x")
-    T, D = x.shape
+    gpu, T, D, xp, ldx = _matrix(x, "x", _FMT)
     dt = x.dtype
-    xp, ldx = _rows(x, "x", T, D, _FMT, gpu)
     yf = _FMT.get(out_dtype or dt)
     if yf is None:
         raise Q36MoEError("out_dtype must be float32 or bfloat16")
     wp = None if w is None else _packed(w, "w", (D,), _F32, gpu)
     bp = None if b is None else _packed(b, "b", (D,), _F32, gpu)
-    y = x.new_empty((T, D), dtype=out_dtype)
+    y = _like(x, out_dtype)
     if a is None:
         h = hp = ap = None
         lda = D
     else:
         ap, lda = _rows(a, "a", T, D, (dt,), gpu)
-        h = x.new_empty((T, D))
+        h = _like(x)
         hp = h.data_ptr()
     rc = lib().q36moe_layernorm(xp, ldx, ap, lda, _FMT[dt], wp, bp, T, D, eps, NORM_RMS if rms else NORM_LAYER, hp, D,
-                                y.data_ptr(), D, yf, _stream())
+                                y.data_ptr(), D, yf, _raw_stream(gpu))
     if rc:
         check(rc, "q36moe_layernorm")
     return y, h
@@ -660,16 +668,16 @@ def layernorm_backward(dy, h, w=None, dres=None, eps=1e-6, rms=False, want_dx=Tr
     (the residual stream's gradient, added to dx) or None -> (dx, dw, db): dx
     [T, D] in h's dtype, dw and db [D] f32; None for what is not wanted (db is,
     by default, for a layer norm)."""
-    gpu = _gpu_of(h, "h")
-    T, D = h.shape
+    gpu, T, D, hp, ldh = _matrix(h, "h", _FMT)
     dt = h.dtype
-    hp, ldh = _rows(h, "h", T, D, _FMT, gpu)
     gp, ldg = _rows(dy, "dy", T, D, _FMT, gpu)
     rp, ldr = (None, D) if dres is None else _rows(dres, "dres", T, D, (dt,), gpu)
     wp = None if w is None else _packed(w, "w", (D,), _F32, gpu)
-    dx = h.new_empty((T, D)) if want_dx else None
-    dw = h.new_empty((D,), dtype=torch.float32) if want_dw else None
-    db = h.new_empty((D,), dtype=torch.float32) if (not rms if want_db is None else want_db) else None
+    dx = _like(h) if want_dx else None
+    dw = (h.new_empty((D,), dtype=torch.float32) if w is None else torch.empty_like(w)) if want_dw else None
+    db = None
+    if not rms if want_db is None else want_db:
+        db = h.new_empty((D,), dtype=torch.float32) if w is None else torch.empty_like(w)
     L = lib()
     ws = wsp = None
     n = 0
@@ -679,7 +687,8 @@ def layernorm_backward(dy, h, w=None, dres=None, eps=1e-6, rms=False, want_dx=Tr
             ws = h.new_empty((n,), dtype=torch.uint8)
             wsp = ws.data_ptr()
     rc = L.q36moe_layernorm_backward(gp, ldg, _FMT[dy.dtype], hp, ldh, rp, ldr, _FMT[dt], wp, T, D, eps,
-                                     NORM_RMS if rms else NORM_LAYER, _ptr(dx), D, _ptr(dw), _ptr(db), wsp, n, _stream())
+                                     NORM_RMS if rms else NORM_LAYER, _ptr(dx), D, _ptr(dw), _ptr(db), wsp, n,
+                                     _raw_stream(gpu))
     if rc:
         check(rc, "q36moe_layernorm_backward")
     return dx, dw, db
@@ -692,9 +701,7 @@ _I32 = (torch.int32,)
 def _router_args(logits, idx, mask, n_expert):
     """What the logits' operators share: GPU, T, experts, picks, and the
     pointers (and row stride) of logits, idx and mask."""
-    gpu = _gpu_of(logits, "logits")
-    T, E = logits.shape
-    lp, ld = _rows(logits, "logits", T, E, _F32, gpu)
+    gpu, T, E, lp, ld = _matrix(logits, "logits", _F32)
     if not isinstance(idx, torch.Tensor) or idx.dim() != 2:
         raise Q36MoEError("idx must be a tensor [T, k]")
     k = idx.shape[1]
@@ -708,7 +715,7 @@ def balance_loss(logits, idx, coef=1.0, mask=None, n_expert=None):
     (0 for padding) or None -> (loss [] f32, counts int32 [n_expert + 1], the
     last one the number of live tokens, psum f32 [n_expert], the sums of the
     tokens' softmax)."""
-    _, T, E, k, lp, ld, ip, mp = _router_args(logits, idx, mask, n_expert)
+    gpu, T, E, k, lp, ld, ip, mp = _router_args(logits, idx, mask, n_expert)
     loss = logits.new_empty(())
     counts = logits.new_empty((E + 1,), dtype=torch.int32)
     psum = logits.new_empty((E,))
@@ -716,7 +723,7 @@ def balance_loss(logits, idx, coef=1.0, mask=None, n_expert=None):
     n = L.q36moe_balance_loss_workspace(T, E)
     ws = logits.new_empty((n,), dtype=torch.uint8) if n else None
     rc = L.q36moe_balance_loss(lp, ld, ip, mp, T, E, k, coef, counts.data_ptr(), psum.data_ptr(), loss.data_ptr(), _ptr(ws),
-                               n, _stream())
+                               n, _raw_stream(gpu))
     if rc:
         check(rc, "q36moe_balance_loss")
     return loss, counts, psum
@@ -732,9 +739,9 @@ def router_topk_backward(logits, idx, dwt=None, scale=1.0, renorm=True, counts=N
     wp = None if dwt is None else _packed(dwt, "dwt", (T, k), _F32, gpu)
     cp = None if counts is None else _packed(counts, "counts", (E + 1,), _I32, gpu)
     sp = None if dloss is None else _packed(dloss, "dloss", (), _F32, gpu)
-    out = logits.new_empty((T, E))
+    out = _like(logits) if E == logits.shape[1] else logits.new_empty((T, E))
     rc = lib().q36moe_router_topk_backward(lp, ld, ip, wp, cp, mp, sp, T, E, k, scale, 1 if renorm else 0, coef,
-                                           out.data_ptr(), E, _stream())
+                                           out.data_ptr(), E, _raw_stream(gpu))
     if rc:
         check(rc, "q36moe_router_topk_backward")
     return out
@@ -745,26 +752,26 @@ def router_logits_backward(w, x, n_expert, dlogits, dshg=None, want_dw=True, wan
     dlogits [T, n_expert] f32 (row stride free) and, with n_rows == n_expert + 1,
     dshg [T] f32 (any stride) -> (dw f32 [n_rows, 2048], dx [T, 2048] in x's
     dtype; None for what is not wanted)."""
-    gpu = _gpu_of(x, "x")
-    T, D = x.shape
+    gpu, T, D, xp, _ = _matrix(x, "x", _FMT)
+    if not x.is_contiguous():
+        raise Q36MoEError("x must be contiguous")
     if not isinstance(w, torch.Tensor) or w.dim() != 2:
         raise Q36MoEError("w must be a tensor [n_rows, 2048]")
     n_rows = w.shape[0]
     wp = _packed(w, "w", (n_rows, D), _F32, gpu)
-    xp = _packed(x, "x", (T, D), _FMT, gpu)
     gp, ld = _rows(dlogits, "dlogits", T, n_expert, _F32, gpu)
     if (dshg is None) != (n_rows == n_expert):
         raise Q36MoEError("dshg goes with the shared gate's row")
     sp, lds = _shg(dshg, T)
     if dshg is not None and dshg.get_device() != gpu:
         raise Q36MoEError(f"dshg must be on cuda:{gpu}")
-    dw = w.new_empty((n_rows, D)) if want_dw else None
-    dx = x.new_empty((T, D)) if want_dx else None
+    dw = torch.empty_like(w) if want_dw else None
+    dx = torch.empty_like(x) if want_dx else None
     L = lib()
     n = L.q36moe_router_logits_backward_workspace(T, n_rows) if want_dw else 0
     ws = x.new_empty((n,), dtype=torch.uint8) if n else None
     rc = L.q36moe_router_logits_backward(wp, n_rows, n_expert, xp, _FMT[x.dtype], T, D, gp, ld, sp, lds, _ptr(dw), _ptr(dx),
-                                         _ptr(ws), n, _stream())
+                                         _ptr(ws), n, _raw_stream(gpu))
     if rc:
         check(rc, "q36moe_router_logits_backward")
     return dw, dx
