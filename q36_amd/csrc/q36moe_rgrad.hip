@@ -392,7 +392,6 @@ __global__ __launch_bounds__(256) void k_logit_grad(LogitGradArgs A) {
 // ---------------------------------------------------------------------------
 typedef float f32x16 __attribute__((ext_vector_type(16)));
 typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
-typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 typedef uint32_t u32x2_t __attribute__((ext_vector_type(2)));
 
 constexpr int kRgD = 2048;
@@ -570,34 +569,35 @@ __global__ __launch_bounds__(256) void k_router_grad_f32(ProductArgs A) {
     }
 }
 
-// ---- dW of many tokens: operands split into bf16 ----
-// v_mfma_f32_32x32x16_bf16 takes 32 cycles for eight times the products of the
-// fp32 MFMA.  An fp32 value is the sum of three bf16 (8 bits each, the rests
-// exact); of the nine products of two such sums the six down to 2^-16 of the
-// largest are formed, what is left out is 2^-24 of each product.  A bf16 x is
-// one piece, which leaves three products.  No scaling: bf16 has fp32's range.
-struct Pieces { bf16x8 p[3]; };
+// ---- many tokens: operands split into f16 ----
+// v_mfma_f32_32x32x16_f16 takes 32 cycles for eight times the products of the
+// fp32 MFMA.  An fp32 value times a power of two that puts the largest of its row
+// or column near the top of f16's range is the sum of two f16 (11 bits each) to
+// 2^-22 of itself, or to 2^-25 of the scaled range's unit where that is more; three
+// of the four products of two such sums give fp32's exactness (the fourth is 2^-22
+// of the first).  A bf16 value is one f16.  Products of three bf16 pieces need no
+// scaling but are six (three with bf16 x): with random operands the chip holds
+// about 1200 TFLOP/s, and dW of 16384 tokens took 93 us with them (58 bf16).
+__device__ __forceinline__ float pow2(int e) { return __uint_as_float((uint32_t)(e + 127) << 23); }
 
-__device__ __forceinline__ Pieces split3(const float (&v)[8]) {
-    Pieces s;
-    float r[8];
-#pragma unroll
-    for (int i = 0; i < 8; i++) r[i] = v[i];
-#pragma unroll
-    for (int k = 0; k < 3; k++) {
-#pragma unroll
-        for (int i = 0; i < 8; i += 2) {
-            const bf16x2 h = __builtin_convertvector((f32x2{r[i], r[i + 1]}), bf16x2);
-            s.p[k][i] = h[0];
-            s.p[k][i + 1] = h[1];
-            const uint32_t u = __builtin_bit_cast(uint32_t, h);
-            r[i] -= bf16_lo(u);
-            r[i + 1] -= bf16_hi(u);
-        }
-    }
-    return s;
+// Exponent e <= 126 (so that 2^e is a float) with amax * 2^e in [2^top, 2^(top+1)),
+// for inf and NaN as if they were 2^128.
+__device__ __forceinline__ int scale_exp(float amax, int top) {
+    return min(top + 127 - (int)(__float_as_uint(amax) >> 23), 126);
 }
 
+// v * scale as NP f16 pieces.
+template <int NP>
+__device__ __forceinline__ void split_f16(const float (&v)[8], float scale, f16x8 (&p)[NP]) {
+#pragma unroll
+    for (int i = 0; i < 8; i++) {
+        const float s = v[i] * scale;
+        p[0][i] = (_Float16)s;
+        if constexpr (NP > 1) p[1][i] = (_Float16)(s - (float)p[0][i]);
+    }
+}
+
+// ---- dW ----
 // Workgroup: 32 MW router rows x 128 columns over the tokens of its split, 8
 // waves as MW x 8 / MW.  Lane L of an operand holds row (column) L % 32 at K
 // elements (tokens) 8 (L / 32)..+7.  A wave reads its rows of the logits'
@@ -606,15 +606,24 @@ __device__ __forceinline__ Pieces split3(const float (&v)[8]) {
 // order, two buffers, one barrier per 64 tokens.  The columns of MFMA tiles 2q
 // and 2q + 1 interleave, so pairs of columns load and store as 8 bytes.
 // The shared gate's row is an fp32 sum beside the conversion of x.
-constexpr int kDwCols = 128, kDwStep = 64;
+//   Scales: a row's (column's) is chosen from its first 64 tokens, whose largest
+// value it puts at 2^10..2^11, and lowered, the sums so far with it, when a later
+// value would pass f16's largest: looked for in each step's loads a step before
+// their use, by a wave alone in its rows, and in the columns by a flag that the
+// workgroup sees behind the barrier.  The sums follow after the products of the
+// values that still had the old scale.
+constexpr int kDwCols = 128, kDwStep = 64, kDwTop = 10;
+constexpr float kF16Max = 65504.0f;
 
 template <int XF, int MW>
 __global__ __launch_bounds__(512) void k_router_dw_split(ProductArgs A) {
     constexpr bool F32 = XF == Q36MOE_FMT_F32;
-    constexpr int NP = F32 ? 3 : 1;           // pieces of x
+    constexpr int NP = F32 ? 2 : 1;           // pieces of x
     constexpr int NT = MW / 2;                // tiles per wave
-    __shared__ __align__(16) bf16x8 sx[2][NP][4][4][64];
-    __shared__ float ssh[8][kDwCols];
+    __shared__ __align__(16) f16x8 sx[2][NP][4][4][64];
+    __shared__ float scol[8][kDwCols];        // columns' maxima, and the gate's sums at the end
+    __shared__ int ecol[kDwCols], shift[kDwCols];
+    __shared__ int flag;
     const int lane = threadIdx.x & 63, half = lane >> 5, c = lane & 31;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), wm = wave % MW, wn = wave / MW;
     const int mblocks = (A.n_expert + 32 * MW - 1) / (32 * MW), tiles = kRgD / kDwCols * mblocks;
@@ -627,13 +636,15 @@ __global__ __launch_bounds__(512) void k_router_dw_split(ProductArgs A) {
     // (its sums are then not stored): no condition in the loop
     const float *gcol = gate ? A.dsh : A.dl;
     const int64_t gstep = gate ? A.ld_sh : A.ld;
+
     f32x16 acc[NT];
 #pragma unroll
     for (int j = 0; j < NT; j++) acc[j] = f32x16{};
     float sg[2] = {0.0f, 0.0f};
     float a[2][4][8];
     uint32_t xr[8][F32 ? 2 : 1];              // tokens t + 8 wave + i, columns n0 + 2 lane, + 1
-    float sh[8];
+    float sh;                                 // the gate's gradient of token t + 8 wave + lane % 8
+    int er, ex[2];                            // exponents of the lane's row and of its columns of x
 
     // Whole steps load through buffers based at the step's first row, with the
     // rows as scalar offsets: no address arithmetic on the vector unit.  In the
@@ -659,8 +670,7 @@ __global__ __launch_bounds__(512) void k_router_dw_split(ProductArgs A) {
 #pragma unroll
                 for (int i = 0; i < 8; i++) xr[i][0] = __builtin_amdgcn_raw_buffer_load_b32(r, lane * 4, i * kRgD * 2, 0);
             }
-#pragma unroll
-            for (int i = 0; i < 8; i++) sh[i] = gcol[(tx + i) * gstep];
+            sh = gcol[(tx + (lane & 7)) * gstep];
         } else {
 #pragma unroll
             for (int i = 0; i < 8; i++) {
@@ -675,10 +685,13 @@ __global__ __launch_bounds__(512) void k_router_dw_split(ProductArgs A) {
                 }
                 xr[i][0] = tx + i < t1 ? v0 : 0u;
                 if constexpr (F32) xr[i][1] = tx + i < t1 ? v1 : 0u;
-                const float v = gcol[tc * gstep];
-                sh[i] = tx + i < t1 ? v : 0.0f;
             }
+            const float v = gcol[min(tx + (lane & 7), t1 - 1) * gstep];
+            sh = tx + (lane & 7) < t1 ? v : 0.0f;
         }
+    };
+    auto x_at = [&](int i, int u) {
+        return F32 ? __uint_as_float(xr[i][F32 ? u : 0]) : u ? bf16_hi(xr[i][0]) : bf16_lo(xr[i][0]);
     };
     auto load_a = [&](int t, float (&av)[4][8], auto WHOLE) {
         if (decltype(WHOLE)::value || t + kDwStep <= t1) {
@@ -700,29 +713,66 @@ __global__ __launch_bounds__(512) void k_router_dw_split(ProductArgs A) {
                 }
         }
     };
-    auto convert = [&](int buf) {             // this wave's tokens of x to LDS
+    auto row_max = [&](const float (&av)[4][8]) {
+        float m = 0.0f;
+#pragma unroll
+        for (int k = 0; k < 4; k++)
+#pragma unroll
+            for (int i = 0; i < 8; i++) m = fmaxf(m, fabsf(av[k][i]));
+        return m;
+    };
+    // the wave's tokens of x to LDS and to the shared gate's sums
+    auto convert = [&](int buf) {
         const int k = wave >> 1, at = (lane & 31) + 32 * (wave & 1), q = lane >> 5;
 #pragma unroll
         for (int u = 0; u < 2; u++) {
             float v[8];
 #pragma unroll
-            for (int i = 0; i < 8; i++)
-                v[i] = F32 ? __uint_as_float(xr[i][F32 ? u : 0]) : u ? bf16_hi(xr[i][0]) : bf16_lo(xr[i][0]);
-            if constexpr (F32) {
-                const Pieces s = split3(v);
+            for (int i = 0; i < 8; i++) v[i] = x_at(i, u);
+            f16x8 p[NP];
+            split_f16<NP>(v, pow2(ex[u]), p);
 #pragma unroll
-                for (int p = 0; p < NP; p++) sx[buf][p][k][2 * q + u][at] = s.p[p];
-            } else {
-                u32x4_u h;
+            for (int n = 0; n < NP; n++) sx[buf][n][k][2 * q + u][at] = p[n];
 #pragma unroll
-                for (int i = 0; i < 4; i++)   // the columns' halves of two tokens side by side
-                    h[i] = __builtin_amdgcn_perm(xr[2 * i + 1][0], xr[2 * i][0], u ? 0x07060302u : 0x05040100u);
-                sx[buf][0][k][2 * q + u][at] = __builtin_bit_cast(bf16x8, h);
-            }
-#pragma unroll
-            for (int i = 0; i < 8; i++) sg[u] = fmaf(sh[i], v[i], sg[u]);
+            for (int i = 0; i < 8; i++) sg[u] = fmaf(__int_as_float(__builtin_amdgcn_readlane(__float_as_int(sh), i)), v[i], sg[u]);
         }
     };
+    auto x_max = [&](float (&m)[2]) {
+        m[0] = m[1] = 0.0f;
+#pragma unroll
+        for (int i = 0; i < 8; i++)
+#pragma unroll
+            for (int u = 0; u < 2; u++) m[u] = fmaxf(m[u], fabsf(x_at(i, u)));
+    };
+    auto check_x = [&]() {                    // does the step in xr fit its scales?
+        float m[2];
+        x_max(m);
+        if (__any(m[0] * pow2(ex[0]) > kF16Max || m[1] * pow2(ex[1]) > kF16Max) && lane == 0) flag = 1;
+    };
+    // the scales of x for the step in xr, lowered where they do not fit (FIRST:
+    // chosen); shift[] holds by how much.  Ends with a barrier.
+    auto fit_x = [&](auto FIRST) {
+        float m[2];
+        x_max(m);
+        *reinterpret_cast<float2 *>(&scol[wave][2 * lane]) = make_float2(m[0], m[1]);
+        lds_barrier();
+#pragma unroll
+        for (int u = 0; u < 2; u++) {
+            float all = scol[0][2 * lane + u];
+#pragma unroll
+            for (int k = 1; k < 8; k++) all = fmaxf(all, scol[k][2 * lane + u]);
+            const int old = ex[u];
+            if (decltype(FIRST)::value || all * pow2(old) > kF16Max) ex[u] = scale_exp(all, kDwTop);
+            if (wave == 0) {
+                ecol[2 * lane + u] = ex[u];
+                shift[2 * lane + u] = decltype(FIRST)::value ? 0 : ex[u] - old;
+            }
+        }
+        if (threadIdx.x == 0) flag = 0;
+        lds_barrier();
+    };
+    auto col_of = [&](int j) { const int q = wn * NT + j; return 64 * (q >> 1) + 2 * c + (q & 1); };
+
     // One step: the products of its 64 tokens from LDS, and beside them, in the
     // 32 cycles that each MFMA runs, the split of the next 16 tokens' gradients,
     // the conversion of the next step's x into the other buffer and the loads of
@@ -731,57 +781,96 @@ __global__ __launch_bounds__(512) void k_router_dw_split(ProductArgs A) {
     // no conditions, which keeps them one block for the scheduler and the waits
     // before a use counted (after a load that may not have been made they are for
     // every load).
-    Pieces s;                                 // of this step's first 16 tokens
-    auto step = [&](int t, int buf, float (&av)[4][8], const float (&an)[4][8], auto STEADY) {
-        constexpr bool ST = decltype(STEADY)::value;
-        constexpr int NM = NP == 3 ? 6 : 3;   // products per tile
-        const bool one = ST || t + kDwStep < t1, two = ST || t + 2 * kDwStep < t1;
-        lds_barrier();
+    f16x8 s[2];                               // of this step's first 16 tokens
+    constexpr int NM = NP + 1;                // products per tile and 16 tokens
+    // the order of a block of K x 16 tokens: LDS reads of a tile (with bf16 x, whose
+    // registers allow it, a tile ahead), then its MFMAs with V vector instructions
+    // behind each (masks: 0x100 LDS read, 0x8 MFMA, 0x2 vector)
+    auto interleave = [&](auto V, auto K) {
+        if constexpr (!F32) __builtin_amdgcn_sched_group_barrier(0x100, NP, 0);
 #pragma unroll
-        for (int k = 0; k < 4; k++) {
-            const Pieces next = split3(k < 3 ? av[k < 3 ? k + 1 : 0] : an[0]);
-            if (k == 0 && one) convert(buf ^ 1);
-            if (k == 1 && two) load_x(t + 2 * kDwStep, STEADY);
-#pragma unroll
-            for (int j = 0; j < NT; j++) {
-                bf16x8 x[NP];
-#pragma unroll
-                for (int p = 0; p < NP; p++) x[p] = sx[buf][p][k][wn * NT + j][lane];
-                // the smallest products first
-#pragma unroll
-                for (int o = 2; o >= 0; o--)
-#pragma unroll
-                    for (int p = 0; p <= o; p++)
-                        if (p < NP) acc[j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(s.p[o - p], x[p], acc[j], 0, 0, 0);
-            }
-            s = next;
-        }
-        if (two) load_a(t + 2 * kDwStep, av, STEADY);
-        // LDS reads of a tile, then its MFMAs with vector instructions between
-        // (masks: 0x100 LDS read, 0x8 MFMA, 0x2 vector)
-        constexpr int V = (4 * 44 + (F32 ? 104 : 40) + 4 * NT * NM - 1) / (4 * NT * NM);
-#pragma unroll
-        for (int k = 0; k < 4 * NT; k++) {
-            if (k == 0) __builtin_amdgcn_sched_group_barrier(0x100, NP, 0);   // one tile ahead
+        for (int k = 0; k < decltype(K)::value * NT; k++) {
             __builtin_amdgcn_sched_group_barrier(0x100, NP, 0);
 #pragma unroll
             for (int m = 0; m < NM; m++) {
                 __builtin_amdgcn_sched_group_barrier(0x8, 1, 0);
-                __builtin_amdgcn_sched_group_barrier(0x2, V, 0);
+                __builtin_amdgcn_sched_group_barrier(0x2, decltype(V)::value, 0);
             }
+        }
+    };
+    auto step = [&](int t, int buf, float (&av)[4][8], const float (&an)[4][8], auto STEADY) {
+        constexpr bool ST = decltype(STEADY)::value;
+        const bool one = ST || t + kDwStep < t1, two = ST || t + 2 * kDwStep < t1;
+        lds_barrier();
+        const bool low = __builtin_amdgcn_readfirstlane(flag);   // the same for all waves
+        if (low) fit_x(std::false_type{});
+        const float f_now = pow2(er);
+        int en = er;
+#pragma unroll
+        for (int k = 0; k < 4; k++) {
+#pragma unroll
+            for (int j = 0; j < NT; j++) {
+                f16x8 x[NP];
+#pragma unroll
+                for (int p = 0; p < NP; p++) x[p] = sx[buf][p][k][wn * NT + j][lane];
+                // the smallest products first
+                acc[j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(s[1], x[0], acc[j], 0, 0, 0);
+                if constexpr (NP > 1) acc[j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(s[0], x[NP - 1], acc[j], 0, 0, 0);
+                acc[j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(s[0], x[0], acc[j], 0, 0, 0);
+            }
+            if (k < 3) {
+                split_f16<2>(av[k < 3 ? k + 1 : 0], f_now, s);
+            } else {   // the next step's, with the scale that fits it
+                float m = row_max(an);
+                m = fmaxf(m, __shfl_xor(m, 32, 64));
+                en = m * f_now > kF16Max ? scale_exp(m, kDwTop) : er;
+                split_f16<2>(an[0], pow2(en), s);
+            }
+            if (k == 0) {
+                if (one) convert(buf ^ 1);
+                if (two) load_x(t + 2 * kDwStep, STEADY);
+                interleave(std::integral_constant<int, (F32 ? 128 : 112) / (NT * NM) + 1>{}, std::integral_constant<int, 1>{});
+                __builtin_amdgcn_sched_barrier(0);   // x's loads no later
+            }
+        }
+        if (two) load_a(t + 2 * kDwStep, av, STEADY);
+        interleave(std::integral_constant<int, 120 / (3 * NT * NM) + 1>{}, std::integral_constant<int, 3>{});
+        if (two) check_x();
+        if (low)
+#pragma unroll
+            for (int j = 0; j < NT; j++) {
+                const int d = shift[col_of(j)];
+#pragma unroll
+                for (int i = 0; i < 16; i++) acc[j][i] = __builtin_ldexpf(acc[j][i], d);
+            }
+        if (__any(en != er)) {
+            const int d = en - er;
+#pragma unroll
+            for (int i = 0; i < 16; i++) {
+                const int di = __shfl(d, c_row(i, lane), 64);
+#pragma unroll
+                for (int j = 0; j < NT; j++) acc[j][i] = __builtin_ldexpf(acc[j][i], di);
+            }
+            er = en;
         }
     };
     load_x(t0, std::false_type{});
     load_a(t0, a[0], std::false_type{});
+    fit_x(std::true_type{});
     convert(0);
     if (t0 + kDwStep < t1) {
         load_x(t0 + kDwStep, std::false_type{});
         load_a(t0 + kDwStep, a[1], std::false_type{});
+        check_x();
     } else {
 #pragma unroll
         for (int i = 0; i < 32; i++) a[1][i >> 3][i & 7] = 0.0f;
     }
-    s = split3(a[0][0]);
+    {
+        const float m = row_max(a[0]);
+        er = scale_exp(fmaxf(m, __shfl_xor(m, 32, 64)), kDwTop);
+    }
+    split_f16<2>(a[0][0], pow2(er), s);
     int t = t0;
 #pragma unroll 1
     for (; t + 4 * kDwStep <= t1; t += 2 * kDwStep) {
@@ -794,58 +883,46 @@ __global__ __launch_bounds__(512) void k_router_dw_split(ProductArgs A) {
         if (t + kDwStep < t1) step(t + kDwStep, 1, a[1], a[0], std::false_type{});
     }
     float *o = A.dw + (size_t)split * A.n_rows * kRgD;
+    int ec[NT];
+#pragma unroll
+    for (int j = 0; j < NT; j++) ec[j] = ecol[col_of(j)];
 #pragma unroll
     for (int i = 0; i < 16; i++) {
-        const int row = r0 + c_row(i, lane);
+        const int row = r0 + c_row(i, lane), e = __shfl(er, c_row(i, lane), 64);
+        float v[NT];
+#pragma unroll
+        for (int j = 0; j < NT; j++) v[j] = __builtin_ldexpf(acc[j][i], -(e + ec[j]));
         if (row < A.n_expert) {
             if constexpr (NT > 1) {
 #pragma unroll
                 for (int j = 0; j < NT; j += 2)
-                    *reinterpret_cast<float2 *>(o + (size_t)row * kRgD + n0 + 32 * (wn * NT + j) + 2 * c) =
-                        make_float2(acc[j][i], acc[j + 1][i]);
+                    *reinterpret_cast<float2 *>(o + (size_t)row * kRgD + n0 + col_of(j)) = make_float2(v[j], v[j + 1]);
             } else {
-                o[(size_t)row * kRgD + n0 + 64 * (wn >> 1) + 2 * c + (wn & 1)] = acc[0][i];
+                o[(size_t)row * kRgD + n0 + col_of(0)] = v[0];
             }
         }
     }
     if (gate) {   // the waves hold the sums over their eighths of the tokens
-        ssh[wave][2 * lane] = sg[0];
-        ssh[wave][2 * lane + 1] = sg[1];
+        __syncthreads();
+        scol[wave][2 * lane] = sg[0];
+        scol[wave][2 * lane + 1] = sg[1];
         __syncthreads();
         if (threadIdx.x < kDwCols) {
-            float v = ssh[0][threadIdx.x];
+            float v = scol[0][threadIdx.x];
 #pragma unroll
-            for (int k = 1; k < 8; k++) v += ssh[k][threadIdx.x];
+            for (int k = 1; k < 8; k++) v += scol[k][threadIdx.x];
             o[(size_t)A.n_expert * kRgD + n0 + threadIdx.x] = v;
         }
     }
 }
 
-// ---- dx of many tokens, up to 256 experts: operands split into f16 ----
-// All of K fits in registers, so each token's gradients and each column of W
-// can be scaled by a power of two that puts the largest at 2^14..2^15: two f16
-// (11 bits each) then hold a value to 2^-22 of itself, or to 2^-40 of the
-// largest where that is more, and three products of v_mfma_f32_32x32x16_f16
-// give fp32's exactness (the fourth is 2^-22 of the first).  The same for a bf16
-// dx: one f16 per operand would be a third of the products, but 2^-10 of each
-// term, which is above the result's own rounding where the terms cancel.
+// ---- dx, up to 256 experts ----
+// All of K fits in registers, so each token's gradients and each column of W are
+// scaled by their own largest, to 2^14..2^15.  The same for a bf16 dx: one f16 per
+// operand would be a third of the products, but 2^-10 of each term, which is above
+// the result's own rounding where the terms cancel.
 // Workgroup: 256 tokens, 32 per wave with their gradients in registers, against
 // its part of the columns, 64 at a time through LDS.
-__device__ __forceinline__ int scale_exp(float amax) {   // amax * 2^this is in [2^14, 2^15)
-    const int e = (int)(__float_as_uint(amax) >> 23);     // 0 for zero and denormals, 255 for inf
-    return 141 - max(e, 1);
-}
-
-template <int NP>
-__device__ __forceinline__ void split_f16(const float (&v)[8], int e, f16x8 (&p)[NP]) {
-#pragma unroll
-    for (int i = 0; i < 8; i++) {
-        const float s = __builtin_ldexpf(v[i], e);
-        p[0][i] = (_Float16)s;
-        if constexpr (NP > 1) p[1][i] = (_Float16)(s - (float)p[0][i]);
-    }
-}
-
 constexpr int kDxRows = 256, kDxCols = 64, kDxStages = kRgD / kDxCols;
 
 template <int XF, int KS>   // K-steps of 16: 8 or 16
@@ -934,10 +1011,10 @@ __global__ __launch_bounds__(512) void k_router_dx_split(ProductArgs A) {
         for (int k = 0; k < KS; k++)
 #pragma unroll
             for (int i = 0; i < 8; i++) m = fmaxf(m, fabsf(raw[k][i]));
-        const int e = scale_exp(fmaxf(m, __shfl_xor(m, 32, 64)));
+        const int e = scale_exp(fmaxf(m, __shfl_xor(m, 32, 64)), 14);
         if (lane < 32) srow[wave][lane] = -e;
 #pragma unroll
-        for (int k = 0; k < KS; k++) split_f16<NP>(raw[k], e, ga[k]);
+        for (int k = 0; k < KS; k++) split_f16<NP>(raw[k], pow2(e), ga[k]);
     }
     for (int st = s0; st < s1; st++) {
         const int n0 = st * kDxCols;
@@ -959,19 +1036,19 @@ __global__ __launch_bounds__(512) void k_router_dx_split(ProductArgs A) {
             m0 = fmaxf(m0, v.x);
             m1 = fmaxf(m1, v.y);
         }
-        const int e0 = scale_exp(m0), e1 = scale_exp(m1);
+        const int e0 = scale_exp(m0, 14), e1 = scale_exp(m1, 14);
 #pragma unroll
         for (int j = 0; j < JW; j++) {
             float v[8];
             f16x8 h[NP];
 #pragma unroll
             for (int i = 0; i < 8; i++) v[i] = wr[j][i].x;
-            split_f16<NP>(v, e0, h);
+            split_f16<NP>(v, pow2(e0), h);
 #pragma unroll
             for (int p = 0; p < NP; p++) sw[p][0][wave * JW + j][lane] = h[p];
 #pragma unroll
             for (int i = 0; i < 8; i++) v[i] = wr[j][i].y;
-            split_f16<NP>(v, e1, h);
+            split_f16<NP>(v, pow2(e1), h);
 #pragma unroll
             for (int p = 0; p < NP; p++) sw[p][1][wave * JW + j][lane] = h[p];
         }

@@ -557,6 +557,33 @@ def test_router_logits_backward_zero_gradients_and_infinities(dev, T):
     assert torch.equal(dw1[keep_r], dw0[keep_r]) and torch.equal(dx1[keep_t], dx0[keep_t])
 
 
+@pytest.mark.parametrize("xt", [F32, BF16])
+def test_router_logits_backward_growing_values(dev, xt):
+    """Values that grow along the tokens by factors of 10^4 at places of their
+    own per row and column (and rows and columns that begin with zeros, or are
+    zero throughout): the sums before and after a jump keep fp32's exactness."""
+    T, E = 2600, 256
+    g = _g(91)
+    d, x, w = _randn(g, T, E + 1), _randn(g, T, 2048), 0.02 * _randn(g, E + 1, 2048)
+    at_d, at_x = torch.randint(0, T, (E + 1,), generator=g), torch.randint(0, T, (2048,), generator=g)
+    tok = torch.arange(T)[:, None]
+    d = torch.where(tok >= at_d, d * 1e4, d * (torch.arange(E + 1) % 5 != 2))
+    x = torch.where(tok >= at_x, x * 1e4, x * (torch.arange(2048) % 7 != 3))
+    d[:, 17], x[:, 100] = 0.0, 0.0
+    d[:, 18] *= 1e-30
+    x[:, 101] *= 1e-30
+    x = x.to(xt)
+    dw, dx = moe.router_logits_backward(w.to(dev), x.to(dev), E, d[:, :E].contiguous().to(dev), d[:, E].to(dev))
+    d64, x64, w64 = d.double(), x.double(), w.double()
+    few = lambda n: (8 + 6 * (n / 3) ** 0.5) * U
+    # the product of the two small ones, 10^-51, is under fp32's range, whose
+    # rounding there is 2^-150
+    _within(dw, d64.T @ x64, few(T) * (d64.abs().T @ x64.abs()) + 2.0 ** -150, "dw")
+    ref = d64 @ w64
+    lost = few(E + 1) + (0 if xt == F32 else 2.0 ** -14)
+    _within(dx, ref, lost * (d64.abs() @ w64.abs()) + HALF[xt] * ref.abs(), "dx")
+
+
 # --------------------------------------------------------------------------
 # all of them
 # --------------------------------------------------------------------------
