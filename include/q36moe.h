@@ -246,9 +246,9 @@ int q36moe_forward_q8(q36moe_ctx *c, const q36moe_weights *w, const uint8_t *xq,
  * learn.  No counterpart in the reference, which only infers.  All of these
  * take device pointers, are asynchronous on `stream`, allocate nothing and
  * may be captured.  A workspace belongs to the caller: it holds nothing
- * between calls, needs no clearing, and must not serve two calls that can
- * run at the same time.  Its size is what the _workspace function gives for
- * the same sizes (0: ws may be NULL).  Outputs do not overlap inputs, but
+ * between calls, needs no clearing, is aligned to 16 bytes, and must not
+ * serve two calls that can run at the same time.  Its size is what the
+ * _workspace function gives for the same sizes (0: ws may be NULL).  Outputs do not overlap inputs, but
  * where stated.  Sums are fp32; the same call gives the same bits. */
 
 /* Residual add and norm.  Rows of d_model (1..16384) elements, row strides
@@ -281,7 +281,8 @@ int q36moe_layernorm_backward(const void *dy, int64_t ld_dy, int y_fmt, const vo
 /* Load of the experts and the loss that balances it.  logits [T][ld] f32,
  * idx [T][k] as q36moe_router_topk gives it (an index outside
  * 0..n_expert-1 is a dropped pick and not counted), mask [T] bytes or NULL:
- * a token with 0 is padding, and nothing of it is read or counted.  With
+ * a token with 0 is padding and counts for nothing, whatever its logits and
+ * picks hold (NaN too).  n_expert <= 256, k <= 8, T * k < 2^31.  With
  * p = softmax(logits[t]) over the n tokens that are left:
  *   counts[e] = picks of e,  counts[n_expert] = n,  psum[e] = sum_t p[e]
  *   loss = coef * n_expert / (k * n^2) * sum_e counts[e] * psum[e]
@@ -303,21 +304,26 @@ int q36moe_balance_loss(const float *logits, int ld, const int32_t *idx, const u
  *   them and dloss its gradient (device pointer, NULL: 1): with
  *   f = counts / (k * n), dloss * coef * n_expert / n * p * (f - sum_e p_e f_e).
  *   counts summed over several GPUs first give the loss of all their tokens.
- * A token with mask 0 gets a row of zeros and nothing of it is read; a pick
- * outside 0..n_expert-1 takes no part; one that stands twice adds up.
+ * A token with mask 0 gets a row of zeros, whatever its logits, picks and
+ * dwt hold; a pick outside 0..n_expert-1 takes no part; one that stands
+ * twice adds up; a pick whose logit is -inf has no weight and no gradient.
  * dlogits [T][ld_d], all n_expert columns of each row. */
 int q36moe_router_topk_backward(const float *logits, int ld, const int32_t *idx, const float *dwt,
                                 const int32_t *counts, const uint8_t *mask, const float *dloss, int T,
                                 int n_expert, int k, float scale, int renorm, float coef, float *dlogits, int ld_d,
                                 void *stream);
 
-/* Gradients of q36moe_router_logits (fp32 products and sums, whatever mode
- * the forward ran in): dlogits [T][ld], and with n_rows == n_expert + 1
- * dshg, token t's at dshg[t * ld_shg] (ld_shg 0 means 1):
+/* Gradients of q36moe_router_logits, to fp32 whatever mode the forward ran
+ * in: dlogits [T][ld] (ld <= 2^22), and with n_rows == n_expert + 1 dshg,
+ * token t's at dshg[t * ld_shg] (ld_shg 0 means 1):
  *   dw[r] = sum_t dlogits[t][r] * x[t],  dx[t] = sum_r dlogits[t][r] * w[r]
  * with the shared gate as the last row.  dw [n_rows][d_model] f32, dx
  * [T][d_model] in x_fmt; either may be NULL (x is read for dw alone, w for
- * dx alone).  d_model == 2048, T <= 2^25.  T = 0 clears dw. */
+ * dx alone).  d_model == 2048, T <= 2^23, x and dx aligned to 4 bytes.  From
+ * some hundred tokens on an operand is the sum of two f16, scaled by its row's
+ * or column's largest value: off by 2^-22 of itself, or 2^-35 of that largest
+ * where that is more.  Every token's x enters dw: one that is not finite makes
+ * it NaN even where its gradients are 0.  T = 0 clears dw. */
 size_t q36moe_router_logits_backward_workspace(int T, int n_rows);
 int q36moe_router_logits_backward(const float *w, int n_rows, int n_expert, const void *x, int x_fmt, int T,
                                   int d_model, const float *dlogits, int ld, const float *dshg, int ld_shg,

@@ -354,7 +354,7 @@ int q36moe_layernorm_backward(const void *dy, int64_t ld_dy, int y_fmt, const vo
     const bool sums = dw || db;
     if (T == 0 && !sums) return Q36MOE_OK;
     if (T > 0 && (!dy || !h)) return Q36MOE_EINVAL;
-    if (T > 1 && sums && (!ws || ws_bytes < q36moe_layernorm_backward_workspace(T, d_model))) return Q36MOE_EINVAL;
+    if (sums && !workspace_ok(ws, ws_bytes, q36moe_layernorm_backward_workspace(T, d_model))) return Q36MOE_EINVAL;
     hipStream_t s = static_cast<hipStream_t>(stream);
     const size_t D = (size_t)d_model;
     const size_t L = D * ((dw ? 1 : 0) + (db ? 1 : 0));

@@ -395,7 +395,7 @@ typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
 typedef uint32_t u32x2_t __attribute__((ext_vector_type(2)));
 
 constexpr int kRgD = 2048;
-constexpr int kMaxRouterT = 1 << 25, kMaxRouterRows = 1 << 20, kMaxRouterLd = 1 << 22;
+constexpr int kMaxRouterT = 1 << 23, kMaxRouterRows = 1 << 20, kMaxRouterLd = 1 << 22;
 
 struct ProductArgs {
     const float *w, *dl, *dsh;   // [n_rows][kRgD]; [T][ld]; the shared gate's column, stride ld_sh
@@ -1085,8 +1085,8 @@ constexpr int kCUs = 256;
 // Tokens from which the split operands pay.  Their time is nearly flat there (two
 // launches of one workgroup per CU, and the sum of dW's splits), that of the fp32
 // tiles grows with the tokens.  us of both gradients, fp32 x (fp32 tiles / split):
-// 256 + 1 rows, 512 tokens 27 / 32, 700 35 / 33, 1024 46 / 36; 128 rows, 700
-// 19 / 22, 1024 24 / 25, 1400 31 / 27; 60 rows, 1024 20 / 25, 1400 27 / 27, 2048 36 / 29.
+// 256 + 1 rows, 512 tokens 27 / 30, 700 35 / 32, 1024 46 / 33; 128 rows, 700
+// 19 / 22, 1024 24 / 25, 1400 31 / 28; 60 rows, 1024 20 / 25, 1400 27 / 27, 2048 36 / 29.
 int split_from(int n_expert) { return n_expert > 128 ? 640 : n_expert > 64 ? 1024 : 1400; }
 
 // Waves along the router rows in k_router_dw_split.
@@ -1152,8 +1152,9 @@ int q36moe_balance_loss(const float *logits, int ld, const int32_t *idx, const u
     if (T < 0 || n_expert < 1 || n_expert > kMaxE || ld < n_expert || k < 1 || k > kMaxK || k > n_expert)
         return Q36MOE_EINVAL;
     if (!counts || !psum || !loss || (T > 0 && (!logits || !idx))) return Q36MOE_EINVAL;
+    if ((int64_t)T * k > INT32_MAX) return Q36MOE_EINVAL;   // counts are 32 bits
     const size_t need = q36moe_balance_loss_workspace(T, n_expert);
-    if (need && (!ws || ws_bytes < need)) return Q36MOE_EINVAL;
+    if (!workspace_ok(ws, ws_bytes, need)) return Q36MOE_EINVAL;
     BalanceArgs A{logits, idx, mask, ld, T, n_expert, k, 0, coef, counts, psum, loss, static_cast<float2 *>(ws)};
     const int nb = T ? balance_groups(T) : 1;
     A.chunk = (int)(((int64_t)T + nb - 1) / nb);
@@ -1208,7 +1209,8 @@ int q36moe_router_logits_backward(const float *w, int n_rows, int n_expert, cons
     }
     if (!dlogits || (dw && !x) || (dx && !w) || (n_rows > n_expert && !dshg)) return Q36MOE_EINVAL;
     const size_t need = dw ? q36moe_router_logits_backward_workspace(T, n_rows) : 0;
-    if (need && (!ws || ws_bytes < need)) return Q36MOE_EINVAL;
+    if (!workspace_ok(ws, ws_bytes, need)) return Q36MOE_EINVAL;
+    if (((uintptr_t)x | (uintptr_t)dx) & 3) return Q36MOE_EINVAL;   // pairs of bf16
     ProductArgs A{};
     A.w = w; A.dl = dlogits; A.dsh = dshg; A.x = x; A.dx = dx;
     A.ld = ld; A.ld_sh = ld_shg ? ld_shg : 1;

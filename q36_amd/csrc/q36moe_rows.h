@@ -21,6 +21,10 @@ typedef uint32_t u32x4_u __attribute__((ext_vector_type(4), aligned(2)));
 typedef float f32x2 __attribute__((ext_vector_type(2)));
 typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
 
+inline bool workspace_ok(const void *ws, size_t bytes, size_t need) {
+    return need == 0 || (ws && bytes >= need && ((uintptr_t)ws & 15) == 0);
+}
+
 int hip_status(hipError_t e) { return e == hipSuccess ? Q36MOE_OK : Q36MOE_EHIP; }
 
 __device__ __forceinline__ float bf16_lo(uint32_t u) { return __uint_as_float(u << 16); }

@@ -64,7 +64,7 @@ def _wide(t, pad, dev, dtype, sentinel=False):
     return buf[:, :D]
 
 
-NORM_SHAPES = [(1, 1), (3, 2), (1, 7), (5, 8), (2, 63), (9, 64), (1, 255), (4, 257), (3, 511), (5, 513), (7, 1023),
+NORM_SHAPES = [(1, 1), (4, 1), (3, 2), (1, 7), (5, 8), (2, 63), (9, 64), (1, 255), (4, 257), (3, 511), (5, 513), (7, 1023),
                (1, 2048), (61, 2048), (2, 2049), (3, 4095), (2, 4097), (2, 8191), (3, 8192), (2, 8193), (2, 16383),
                (1, 16384), (1030, 130)]
 

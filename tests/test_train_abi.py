@@ -42,7 +42,7 @@ LNB = dict(dy=P, ld_dy=64, y_fmt=0, h=P, ld_h=64, dres=None, ld_dres=0, x_fmt=0,
     {"T": -1}, {"d": 0}, {"d": 16385, "ld_dy": 20000, "ld_h": 20000, "ld_dx": 20000}, {"eps": F(float("nan"))}, {"kind": 7},
     {"x_fmt": 3}, {"y_fmt": 2}, {"ld_dy": 63}, {"ld_h": 63}, {"ld_dx": 63}, {"dres": P, "ld_dres": 63},
     {"dres": P, "ld_dres": 64, "dx": None}, {"dx": None, "dw": None, "db": None}, {"dy": None}, {"h": None}, {"ws": None},
-    {"ws_bytes": 4 * 2 * 64 * 4 - 1}])
+    {"ws_bytes": 4 * 2 * 64 * 4 - 1}, {"ws": ctypes.c_void_p(72)}])
 def test_layernorm_backward_refuses(L, change):
     assert _call(L.q36moe_layernorm_backward, LNB, **change) == -22
 
@@ -53,7 +53,8 @@ BAL = dict(logits=P, ld=256, idx=P, mask=None, T=4, E=256, k=8, coef=F(1.0), cou
 
 @pytest.mark.parametrize("change", [
     {"T": -1}, {"E": 0}, {"E": 257, "ld": 257}, {"ld": 255}, {"k": 0}, {"k": 9}, {"E": 4, "k": 5}, {"logits": None},
-    {"idx": None}, {"counts": None}, {"psum": None}, {"loss": None}, {"T": 100000}, {"T": 100000, "ws": P, "n": 64}])
+    {"idx": None}, {"counts": None}, {"psum": None}, {"loss": None}, {"T": 100000}, {"T": 100000, "ws": P, "n": 64},
+    {"T": 100000, "ws": ctypes.c_void_p(72), "n": 1 << 30}, {"T": 1 << 28, "ws": P, "n": 1 << 30}])
 def test_balance_loss_refuses(L, change):
     assert _call(L.q36moe_balance_loss, BAL, **change) == -22
 
@@ -74,9 +75,11 @@ RLB = dict(w=P, n_rows=257, E=256, x=P, x_fmt=0, T=4, d=2048, dlogits=P, ld=256,
 
 
 @pytest.mark.parametrize("change", [
-    {"T": -1}, {"T": (1 << 25) + 1}, {"d": 2000}, {"E": 0}, {"n_rows": 255}, {"n_rows": 258}, {"ld": 255}, {"x_fmt": 2},
+    {"T": -1}, {"T": (1 << 23) + 1}, {"d": 2000}, {"E": 0}, {"n_rows": 255}, {"n_rows": 258}, {"ld": 255}, {"x_fmt": 2},
     {"dw": None, "dx": None}, {"dlogits": None}, {"x": None}, {"w": None}, {"dshg": None}, {"ld_shg": -1},
-    {"T": 100000, "ws": None}, {"T": 100000, "n": 1024}])
+    {"T": 100000, "ws": None}, {"T": 100000, "n": 1024},
+    {"T": 100000, "ws": ctypes.c_void_p(72)}, {"ld": (1 << 22) + 1}, {"x": ctypes.c_void_p(66), "x_fmt": 1},
+    {"dx": ctypes.c_void_p(66), "x_fmt": 1}, {"n_rows": (1 << 20) + 1, "E": 1 << 20, "ld": 1 << 20}])
 def test_router_logits_backward_refuses(L, change):
     assert _call(L.q36moe_router_logits_backward, RLB, **change) == -22
 
@@ -98,8 +101,8 @@ def test_workspaces_grow_no_further_than_the_chip(L):
     assert b(1, 256) == 0 and b(0, 256) == 0 and b(1000, 257) == 0
     assert 0 < b(1 << 15, 256) <= b((1 << 31) - 1, 256) < 1 << 22
     r = L.q36moe_router_logits_backward_workspace
-    assert r(0, 257) == 0 and r((1 << 25) + 1, 257) == 0 and r(4, 0) == 0
-    assert r(1 << 25, 257) < 1 << 28
+    assert r(0, 257) == 0 and r((1 << 23) + 1, 257) == 0 and r(4, 0) == 0
+    assert r(1 << 23, 257) < 1 << 28
 
 
 def test_python_refuses_host_tensors():
