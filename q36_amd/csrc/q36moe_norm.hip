@@ -71,6 +71,9 @@ struct Cols {
     }
 };
 
+// One row per workgroup of NW waves (four rows of a wave each where NW is 1).
+// Measured with residual: 4006 bf16 rows of 2048 13 us (5.0 TB/s), 16384 fp32 rows
+// 94 us (5.7 TB/s); 4096 fp32 rows with bf16 y by 1 / 2 / 4 waves 28 / 25 / 24 us.
 template <int XF, int YF, int VEC, int NW, int NV>
 __global__ __launch_bounds__(NW == 1 ? 256 : 64 * NW) void k_layernorm(NormArgs A) {
     constexpr int TPR = 64 * NW, RPB = NW == 1 ? 4 : 1;

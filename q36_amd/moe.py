@@ -655,7 +655,7 @@ def layernorm(x, w=None, b=None, a=None, eps=1e-6, rms=False, out_dtype=None):
         ap, lda = _rows(a, "a", T, D, (dt,), gpu)
         h = _like(x)
         hp = h.data_ptr()
-    rc = lib().q36moe_layernorm(xp, ldx, ap, lda, _FMT[dt], wp, bp, T, D, eps, NORM_RMS if rms else NORM_LAYER, hp, D,
+    rc = lib().q36moe_layernorm(xp, ldx, ap, lda, _FMT[dt], wp, bp, T, D, float(eps), NORM_RMS if rms else NORM_LAYER, hp, D,
                                 y.data_ptr(), D, yf, _raw_stream(gpu))
     if rc:
         check(rc, "q36moe_layernorm")
@@ -686,7 +686,7 @@ def layernorm_backward(dy, h, w=None, dres=None, eps=1e-6, rms=False, want_dx=Tr
         if n:
             ws = h.new_empty((n,), dtype=torch.uint8)
             wsp = ws.data_ptr()
-    rc = L.q36moe_layernorm_backward(gp, ldg, _FMT[dy.dtype], hp, ldh, rp, ldr, _FMT[dt], wp, T, D, eps,
+    rc = L.q36moe_layernorm_backward(gp, ldg, _FMT[dy.dtype], hp, ldh, rp, ldr, _FMT[dt], wp, T, D, float(eps),
                                      NORM_RMS if rms else NORM_LAYER, _ptr(dx), D, _ptr(dw), _ptr(db), wsp, n,
                                      _raw_stream(gpu))
     if rc:
@@ -702,6 +702,8 @@ def _router_args(logits, idx, mask, n_expert):
     """What the logits' operators share: GPU, T, experts, picks, and the
     pointers (and row stride) of logits, idx and mask."""
     gpu, T, E, lp, ld = _matrix(logits, "logits", _F32)
+    if n_expert and n_expert > E:
+        raise Q36MoEError(f"logits have {E} columns, n_expert is {n_expert}")
     if not isinstance(idx, torch.Tensor) or idx.dim() != 2:
         raise Q36MoEError("idx must be a tensor [T, k]")
     k = idx.shape[1]
@@ -722,7 +724,7 @@ def balance_loss(logits, idx, coef=1.0, mask=None, n_expert=None):
     L = lib()
     n = L.q36moe_balance_loss_workspace(T, E)
     ws = logits.new_empty((n,), dtype=torch.uint8) if n else None
-    rc = L.q36moe_balance_loss(lp, ld, ip, mp, T, E, k, coef, counts.data_ptr(), psum.data_ptr(), loss.data_ptr(), _ptr(ws),
+    rc = L.q36moe_balance_loss(lp, ld, ip, mp, T, E, k, float(coef), counts.data_ptr(), psum.data_ptr(), loss.data_ptr(), _ptr(ws),
                                n, _raw_stream(gpu))
     if rc:
         check(rc, "q36moe_balance_loss")
@@ -740,8 +742,8 @@ def router_topk_backward(logits, idx, dwt=None, scale=1.0, renorm=True, counts=N
     cp = None if counts is None else _packed(counts, "counts", (E + 1,), _I32, gpu)
     sp = None if dloss is None else _packed(dloss, "dloss", (), _F32, gpu)
     out = _like(logits) if E == logits.shape[1] else logits.new_empty((T, E))
-    rc = lib().q36moe_router_topk_backward(lp, ld, ip, wp, cp, mp, sp, T, E, k, scale, 1 if renorm else 0, coef,
-                                           out.data_ptr(), E, _raw_stream(gpu))
+    rc = lib().q36moe_router_topk_backward(lp, ld, ip, wp, cp, mp, sp, T, E, k, float(scale), 1 if renorm else 0,
+                                           float(coef), out.data_ptr(), E, _raw_stream(gpu))
     if rc:
         check(rc, "q36moe_router_topk_backward")
     return out

@@ -522,9 +522,10 @@ def test_router_logits_backward(dev, T, E, shared, xt):
     _within(dx, ref_x, lost * mag_x + HALF[xt] * ref_x.abs(), "dx")
 
 
-def test_router_logits_backward_wants_and_empty(dev):
+@pytest.mark.parametrize("T", [50, 1500])
+def test_router_logits_backward_wants_and_empty(dev, T):
     g = _g(2)
-    w, x, d = _randn(g, 20, 2048).to(dev), _randn(g, 50, 2048).to(dev), _randn(g, 50, 20).to(dev)
+    w, x, d = _randn(g, 20, 2048).to(dev), _randn(g, T, 2048).to(dev), _randn(g, T, 20).to(dev)
     dw, dx = moe.router_logits_backward(w, x, 20, d)
     a, b = moe.router_logits_backward(w, x, 20, d, want_dw=False)
     assert a is None and torch.equal(b, dx)
@@ -532,6 +533,9 @@ def test_router_logits_backward_wants_and_empty(dev):
     assert b is None and torch.equal(a, dw)
     dw, dx = moe.router_logits_backward(w, x[:0], 20, d[:0])
     assert dx.shape == (0, 2048) and not bool(dw.any())
+    w, x = torch.zeros(257, 2048, device=dev), torch.zeros(0, 2048, device=dev)
+    dw, _ = moe.router_logits_backward(w, x, 256, torch.zeros(0, 256, device=dev), torch.zeros(0, device=dev))
+    assert dw.shape == (257, 2048) and not bool(dw.any())
     with pytest.raises(moe.Q36MoEError):
         moe.router_logits_backward(w, x, 19, d[:, :19])          # a row of the shared gate without its gradient
     with pytest.raises(moe.Q36MoEError):
@@ -652,6 +656,38 @@ def test_two_streams_at_once(dev):
             assert torch.equal(t, r)
 
 
+def test_offsets_past_32_bits(dev):
+    """Rows so far apart that their offsets need more than 32 bits, in elements
+    and in bytes, give what the same rows give side by side."""
+    g = _g(61)
+
+    def far(rows, gap, dtype):
+        T, n = rows.shape
+        buf = torch.empty((T - 1) * gap + n, dtype=dtype, device=dev).as_strided((T, n), (gap, 1))
+        return buf.copy_(rows.to(dev))
+
+    x, dy = _randn(g, 4, 700).to(BF16), _randn(g, 4, 700)
+    xf, gf = far(x, 2 ** 30 + 12, BF16), far(dy, 2 ** 29 + 4, F32)
+    x, dy = x.to(dev), dy.to(dev)
+    for a, b in ((moe.layernorm(xf, a=xf)[0], moe.layernorm(x, a=x)[0]),
+                 *zip(moe.layernorm_backward(gf, xf, dres=xf), moe.layernorm_backward(dy, x, dres=x))):
+        assert torch.equal(a, b)
+    del xf, gf
+    l, idx = _routing(g, 6, 130, 4)
+    lf, idx, dwt = far(l, 2 ** 29 + 4, F32), idx.to(dev), _randn(g, 6, 4).to(dev)
+    l = l.to(dev)
+    got, want = moe.balance_loss(lf, idx), moe.balance_loss(l, idx)
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
+    assert torch.equal(moe.router_topk_backward(lf, idx, dwt, counts=want[1]), moe.router_topk_backward(l, idx, dwt, counts=want[1]))
+    del lf
+    for T in (600, 700):
+        w, x, d = (0.02 * _randn(g, 200, 2048)).to(dev), _randn(g, T, 2048).to(dev), _randn(g, T, 200)
+        df = far(d, 2 ** 22, F32)
+        for a, b in zip(moe.router_logits_backward(w, x, 200, df), moe.router_logits_backward(w, x, 200, d.to(dev))):
+            assert torch.equal(a, b)
+        del df
+
+
 def test_python_refusals(dev):
     x = torch.zeros(4, 64, device=dev)
     idx = torch.zeros(4, 3, dtype=torch.int32, device=dev)
@@ -664,7 +700,9 @@ def test_python_refusals(dev):
            lambda: moe.layernorm_backward(x.cpu(), x),
            lambda: moe.balance_loss(x.double(), idx), lambda: moe.balance_loss(x, idx.long()), lambda: moe.balance_loss(x, idx[:3]),
            lambda: moe.balance_loss(x, idx, mask=torch.ones(3, dtype=torch.bool, device=dev)),
-           lambda: moe.balance_loss(x, idx, n_expert=65), lambda: moe.balance_loss(torch.zeros(4, 257, device=dev), idx),
+           lambda: moe.balance_loss(x, idx, n_expert=65), lambda: moe.balance_loss(x[:, :40], idx, n_expert=45),
+           lambda: moe.router_topk_backward(x[:, :40], idx, x[:, :3].contiguous(), n_expert=45),
+           lambda: moe.balance_loss(torch.zeros(4, 257, device=dev), idx),
            lambda: moe.balance_loss(x, torch.zeros(4, 9, dtype=torch.int32, device=dev)),
            lambda: moe.balance_loss(x, torch.zeros(4, 6, dtype=torch.int32, device=dev)[:, ::2]),
            lambda: moe.router_topk_backward(x, idx), lambda: moe.router_topk_backward(x, idx, x[:, :2]),
