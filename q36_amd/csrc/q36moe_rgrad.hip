@@ -614,8 +614,8 @@ __device__ __forceinline__ void split_f16(const float (&v)[8], float scale, f16x
 // their use, by a wave alone in its rows, and in the columns by a flag that the
 // workgroup sees behind the barrier.  The sums follow after the products of the
 // values that still had the old scale.
-//   4096 / 16384 fp32 tokens and 256 rows 32 / 72 us with the sum of the splits
-// (bf16 x 27 / 55).  The splits' parts, 33.5 MB at 256 rows, are one tile per CU.
+//   4096 / 16384 fp32 tokens and 256 rows 33 / 73 us with the sum of the splits
+// (bf16 x 28 / 55).  The splits' parts, 33.5 MB at 256 rows, are one tile per CU.
 constexpr int kDwCols = 128, kDwStep = 64, kDwTop = 10;
 constexpr float kF16Max = 65504.0f;
 
@@ -627,7 +627,9 @@ __global__ __launch_bounds__(512) void k_router_dw_split(ProductArgs A) {
     __shared__ __align__(16) f16x8 sx[2][NP][4][4][64];
     __shared__ float scol[8][kDwCols];        // columns' maxima, and the gate's sums at the end
     __shared__ int ecol[kDwCols], shift[kDwCols];
-    __shared__ int flag;
+    // per x buffer, as a wave may end a step, and set the next one's, while another
+    // has yet to read this one's
+    __shared__ int flag[2];
     const int lane = threadIdx.x & 63, half = lane >> 5, c = lane & 31;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), wm = wave % MW, wn = wave / MW;
     const int mblocks = (A.n_expert + 32 * MW - 1) / (32 * MW), tiles = kRgD / kDwCols * mblocks;
@@ -748,14 +750,14 @@ __global__ __launch_bounds__(512) void k_router_dw_split(ProductArgs A) {
 #pragma unroll
             for (int u = 0; u < 2; u++) m[u] = fmaxf(m[u], fabsf(x_at(i, u)));
     };
-    auto check_x = [&]() {                    // does the step in xr fit its scales?
+    auto check_x = [&](int buf) {             // does the step in xr fit its scales? asked in the step of buf
         float m[2];
         x_max(m);
-        if (__any(m[0] * pow2(ex[0]) > kF16Max || m[1] * pow2(ex[1]) > kF16Max) && lane == 0) flag = 1;
+        if (m[0] * pow2(ex[0]) > kF16Max || m[1] * pow2(ex[1]) > kF16Max) flag[buf] = 1;
     };
     // the scales of x for the step in xr, lowered where they do not fit (FIRST:
     // chosen); shift[] holds by how much.  Ends with a barrier.
-    auto fit_x = [&](auto FIRST) {
+    auto fit_x = [&](int buf, auto FIRST) {
         float m[2];
         x_max(m);
         *reinterpret_cast<float2 *>(&scol[wave][2 * lane]) = make_float2(m[0], m[1]);
@@ -772,7 +774,10 @@ __global__ __launch_bounds__(512) void k_router_dw_split(ProductArgs A) {
                 shift[2 * lane + u] = decltype(FIRST)::value ? 0 : ex[u] - old;
             }
         }
-        if (threadIdx.x == 0) flag = 0;
+        if (wave == 0) {
+            flag[buf] = 0;
+            if (decltype(FIRST)::value) flag[buf ^ 1] = 0;
+        }
         lds_barrier();
     };
     auto col_of = [&](int j) { const int q = wn * NT + j; return 64 * (q >> 1) + 2 * c + (q & 1); };
@@ -806,8 +811,8 @@ __global__ __launch_bounds__(512) void k_router_dw_split(ProductArgs A) {
         constexpr bool ST = decltype(STEADY)::value;
         const bool one = ST || t + kDwStep < t1, two = ST || t + 2 * kDwStep < t1;
         lds_barrier();
-        const bool low = __builtin_amdgcn_readfirstlane(flag);   // the same for all waves
-        if (low) fit_x(std::false_type{});
+        const bool low = __builtin_amdgcn_readfirstlane(flag[buf]);   // the same for all waves
+        if (low) fit_x(buf, std::false_type{});
         const float f_now = pow2(er);
         int en = er;
 #pragma unroll
@@ -839,7 +844,7 @@ __global__ __launch_bounds__(512) void k_router_dw_split(ProductArgs A) {
         }
         if (two) load_a(t + 2 * kDwStep, av, STEADY);
         interleave(std::integral_constant<int, 120 / (3 * NT * NM) + 1>{}, std::integral_constant<int, 3>{});
-        if (two) check_x();
+        if (two) check_x(buf ^ 1);
         if (low)
 #pragma unroll
             for (int j = 0; j < NT; j++) {
@@ -860,12 +865,12 @@ __global__ __launch_bounds__(512) void k_router_dw_split(ProductArgs A) {
     };
     load_x(t0, std::false_type{});
     load_a(t0, a[0], std::false_type{});
-    fit_x(std::true_type{});
+    fit_x(0, std::true_type{});
     convert(0);
     if (t0 + kDwStep < t1) {
         load_x(t0 + kDwStep, std::false_type{});
         load_a(t0 + kDwStep, a[1], std::false_type{});
-        check_x();
+        check_x(0);
     } else {
 #pragma unroll
         for (int i = 0; i < 32; i++) a[1][i >> 3][i & 7] = 0.0f;
@@ -911,11 +916,12 @@ __global__ __launch_bounds__(512) void k_router_dw_split(ProductArgs A) {
         scol[wave][2 * lane] = sg[0];
         scol[wave][2 * lane + 1] = sg[1];
         __syncthreads();
-        if (threadIdx.x < kDwCols) {
-            float v = scol[0][threadIdx.x];
+        const int col = 64 * wave + lane;
+        if (col < kDwCols) {
+            float v = scol[0][col];
 #pragma unroll
-            for (int k = 1; k < 8; k++) v += scol[k][threadIdx.x];
-            o[(size_t)A.n_expert * kRgD + n0 + threadIdx.x] = v;
+            for (int k = 1; k < 8; k++) v += scol[k][col];
+            o[(size_t)A.n_expert * kRgD + n0 + col] = v;
         }
     }
 }
@@ -927,7 +933,7 @@ __global__ __launch_bounds__(512) void k_router_dw_split(ProductArgs A) {
 // the result's own rounding where the terms cancel.
 // Workgroup: 256 tokens, 32 per wave with their gradients in registers, against
 // its part of the columns, 64 at a time through LDS.  4096 / 16384 fp32 tokens and
-// 256 rows 23 / 63 us; the products alone, at the 1200 TFLOP/s that the chip holds
+// 256 rows 24 / 64 us; the products alone, at the 1200 TFLOP/s that the chip holds
 // on random operands, 11 / 43.
 constexpr int kDxRows = 256, kDxCols = 64, kDxStages = kRgD / kDxCols;
 
