@@ -702,12 +702,14 @@ def _router_args(logits, idx, mask, n_expert):
     """What the logits' operators share: GPU, T, experts, picks, and the
     pointers (and row stride) of logits, idx and mask."""
     gpu, T, E, lp, ld = _matrix(logits, "logits", _F32)
-    if n_expert and n_expert > E:
+    if n_expert is None:
+        n_expert = E
+    elif not 1 <= n_expert <= E:
         raise Q36MoEError(f"logits have {E} columns, n_expert is {n_expert}")
     if not isinstance(idx, torch.Tensor) or idx.dim() != 2:
         raise Q36MoEError("idx must be a tensor [T, k]")
     k = idx.shape[1]
-    return (gpu, T, n_expert or E, k, lp, ld, _packed(idx, "idx", (T, k), _I32, gpu),
+    return (gpu, T, n_expert, k, lp, ld, _packed(idx, "idx", (T, k), _I32, gpu),
             None if mask is None else _packed(mask, "mask", (T,), _MASK, gpu))
 
 

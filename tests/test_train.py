@@ -701,6 +701,7 @@ def test_python_refusals(dev):
            lambda: moe.balance_loss(x.double(), idx), lambda: moe.balance_loss(x, idx.long()), lambda: moe.balance_loss(x, idx[:3]),
            lambda: moe.balance_loss(x, idx, mask=torch.ones(3, dtype=torch.bool, device=dev)),
            lambda: moe.balance_loss(x, idx, n_expert=65), lambda: moe.balance_loss(x[:, :40], idx, n_expert=45),
+           lambda: moe.balance_loss(x, idx, n_expert=0), lambda: moe.balance_loss(x, idx, n_expert=-2),
            lambda: moe.router_topk_backward(x[:, :40], idx, x[:, :3].contiguous(), n_expert=45),
            lambda: moe.balance_loss(torch.zeros(4, 257, device=dev), idx),
            lambda: moe.balance_loss(x, torch.zeros(4, 9, dtype=torch.int32, device=dev)),
