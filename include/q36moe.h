@@ -322,8 +322,9 @@ int q36moe_router_topk_backward(const float *logits, int ld, const int32_t *idx,
  * dx alone).  d_model == 2048, T <= 2^23, x and dx aligned to 4 bytes.  From
  * some hundred tokens on an operand is the sum of two f16, scaled by its row's
  * or column's largest value: off by 2^-22 of itself, or 2^-35 of that largest
- * where that is more.  Every token's x enters dw: one that is not finite makes
- * it NaN even where its gradients are 0.  T = 0 clears dw. */
+ * where that is more.  Every token's x enters dw, padding's too: one that is not
+ * finite makes it NaN even where its gradients are 0, and one 2^13 times its
+ * column's others begins to cost those precision.  T = 0 clears dw. */
 size_t q36moe_router_logits_backward_workspace(int T, int n_rows);
 int q36moe_router_logits_backward(const float *w, int n_rows, int n_expert, const void *x, int x_fmt, int T,
                                   int d_model, const float *dlogits, int ld, const float *dshg, int ld_shg,
